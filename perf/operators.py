@@ -208,7 +208,7 @@ def _prepare_adamw(case, gen):
     arena = {"p": fill(0.02).to(dtype), "g": fill(1e-3).to(dtype)}
     if case["dtype"] == "bf16":  # the 16 bits of the fp32 weight below its bf16 rounding
         low = torch.randint(-32768, 32768, (total,), device="cuda", generator=gen)
-        arena["low"] = (low * inside).to(torch.int16)
+        arena["low"] = (low * (arena["p"] != 0)).to(torch.int16)  # with a zero, negative ones would not be a number
     if case["bits"] == 32:
         arena |= {"m": fill(3e-4), "v": fill(1e-3).square()}
     else:
