@@ -1,0 +1,179 @@
+"""Token-policy operators on the CPU: the PyTorch path against 64-bit definitions, gradients against differences, and
+the refusals."""
+
+import pytest
+import torch
+
+import token_oracle as oracle
+from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
+                                           token_policy_loss_grad)
+
+
+def _case(shape=(5, 7), vocab=11, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(*shape, vocab, generator=g) * 2).to(dtype)
+    tokens = torch.randint(vocab, shape, generator=g)
+    old = torch.randn(shape, generator=g) * 0.3 - 2
+    adv, ref = torch.randn(shape, generator=g), torch.randn(shape, generator=g) * 0.3 - 2
+    mask = torch.rand(shape, generator=g) > 0.3
+    return logits, tokens, old, adv, ref, mask
+
+
+@pytest.mark.parametrize("kind", ["k1", "k2", "k3"])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_policy_loss_and_gradient_match_the_definition(kind, reduction):
+    logits, tokens, old, adv, ref, mask = _case()
+    out, grad = token_policy_loss_grad(logits, tokens, old, adv, ref_logp=ref, mask=mask, clip_high=0.3, kl_coef=0.1,
+                                       kl_estimator=kind, entropy_coef=0.02, temperature=0.7, reduction=reduction,
+                                       grad_scale=3.0)
+    loss, stats, logp, da, db = oracle.policy(logits, tokens, old, adv, ref, mask, lo=0.8, hi=1.3, kl_coef=0.1,
+                                              kind=kind, entropy_coef=0.02, temperature=0.7, mean=reduction == "mean")
+    assert abs(out.loss - loss) < 1e-5 * (1 + abs(loss))
+    for got, want in zip(out[1:5], stats):
+        assert abs(got - want) < 1e-5 * (1 + abs(want))
+    assert torch.allclose(out.logp.double(), logp, atol=1e-5)
+    want, bound = oracle.logits_grad(logits, tokens, mask, 0.7, 3 * da, 3 * db)
+    assert ((grad - want).abs() <= bound + oracle.rounding(want, torch.float32)).all()
+    auto = logits.clone().requires_grad_()
+    (3 * token_policy_loss(auto, tokens, old, adv, ref_logp=ref, mask=mask, clip_high=0.3, kl_coef=0.1,
+                           kl_estimator=kind, entropy_coef=0.02, temperature=0.7, reduction=reduction).loss).backward()
+    assert torch.allclose(auto.grad, grad, atol=1e-6)
+
+
+def test_policy_gradient_matches_differences():
+    logits, tokens, old, adv, ref, mask = _case((3, 4), 6, seed=3)
+    z = logits.double()
+
+    def loss(x):
+        return oracle.policy(x, tokens, old, adv, ref, mask, lo=0.8, hi=1.2, kl_coef=0.2, kind="k3", entropy_coef=0.05,
+                             temperature=1.3)[0]
+
+    _, grad = token_policy_loss_grad(logits, tokens, old, adv, ref_logp=ref, mask=mask, kl_coef=0.2, entropy_coef=0.05,
+                                     temperature=1.3)
+    h = 1e-6
+    for i in range(3):
+        for j in range(4):
+            for c in range(6):
+                up, down = z.clone(), z.clone()
+                up[i, j, c] += h
+                down[i, j, c] -= h
+                # central differences: h^2 / 6 times a third derivative of order one, and 2^-52 / h of rounding
+                assert abs(grad[i, j, c].item() - (loss(up) - loss(down)) / (2 * h)) < 1e-6
+
+
+def test_masked_rows_hold_anything():
+    logits, tokens, old, adv, ref, mask = _case()
+    spoiled = logits.clone()
+    spoiled[~mask] = float("nan")
+    tokens = torch.where(mask, tokens, -100)
+    old = torch.where(mask, old, float("inf"))
+    a = token_policy_loss_grad(logits, tokens, old, adv, ref_logp=ref, kl_coef=0.1)
+    b = token_policy_loss_grad(spoiled, tokens, old, adv, ref_logp=ref, kl_coef=0.1)
+    for x, y in zip((*a[0], a[1]), (*b[0], b[1])):
+        assert torch.equal(x, y)
+    assert (b[1][~mask] == 0).all() and torch.isfinite(b[1]).all()
+
+
+def test_no_counted_row():
+    logits, tokens, old, adv, *_ = _case()
+    out, grad = token_policy_loss_grad(logits, tokens, old, adv, mask=torch.zeros(5, 7))
+    assert out.loss == 0 and (grad == 0).all()
+    logp, entropy = token_logprobs(logits, torch.full_like(tokens, 11))
+    assert (logp == 0).all() and (entropy == 0).all()
+
+
+@pytest.mark.parametrize("kind,smoothing", [("sigmoid", 0.0), ("sigmoid", 0.1), ("hinge", 0.0), ("ipo", 0.0)])
+@pytest.mark.parametrize("average", [False, True])
+def test_preference_matches_the_definition(kind, smoothing, average):
+    logits, tokens, _, _, _, mask = _case((6, 7), seed=1)
+    ref = torch.linspace(-20, -12, 6) if not average else torch.linspace(-3, -2, 6)
+    out, grad = preference_loss_grad(logits, tokens, ref, mask=mask, beta=0.2, loss_type=kind, label_smoothing=smoothing,
+                                     average=average)
+    loss, lps, rewards, da = oracle.preference(logits, tokens, ref, [(7 * i, 7 * i + 7) for i in range(6)], mask,
+                                               beta=0.2, smoothing=smoothing, kind=kind, average=average)
+    assert abs(out.loss - loss) < 1e-5 * (1 + abs(loss))
+    assert torch.allclose(out.seq_logps.double(), lps, atol=1e-4)
+    assert torch.allclose(torch.stack([out.chosen_rewards, out.rejected_rewards], 1).flatten().double(), rewards,
+                          atol=1e-4)
+    want, bound = oracle.logits_grad(logits, tokens, mask, 1.0, da, 0 * da)
+    assert ((grad - want).abs() <= 2 * bound + 1e-5 * want.abs()).all()
+    # packed rows with offsets are the same sequences
+    packed, packed_grad = preference_loss_grad(logits.flatten(0, 1), tokens.flatten(), ref, mask=mask.flatten(),
+                                               offsets=torch.arange(0, 43, 7), beta=0.2, loss_type=kind,
+                                               label_smoothing=smoothing, average=average)
+    assert torch.allclose(packed.loss, out.loss) and torch.allclose(packed_grad.view_as(grad), grad, atol=1e-7)
+
+
+def test_empty_inputs():
+    logits, tokens = torch.zeros(0, 5), torch.zeros(0, dtype=torch.long)
+    none = torch.zeros(0)
+    assert token_logprobs(logits, tokens)[0].shape == (0,)
+    out, grad = token_policy_loss_grad(logits, tokens, none, none)
+    assert out.loss == 0 and grad.shape == (0, 5)
+    out, grad = preference_loss_grad(logits, tokens, none, offsets=torch.zeros(1, dtype=torch.long))
+    assert out.loss == 0 and out.chosen_rewards.shape == (0,)
+
+
+REFUSALS = [
+    (TypeError, "logits must be", dict(logits=lambda x: x.double())),
+    (ValueError, r"\[rows, V\]", dict(logits=lambda x: x[0, 0])),
+    (ValueError, "columns", dict(logits=lambda x: x.transpose(1, 2).contiguous().transpose(1, 2))),
+    (TypeError, "tokens must be", dict(tokens=lambda x: x.short())),
+    (ValueError, "tokens must have the shape", dict(tokens=lambda x: x[:, 1:])),
+    (TypeError, "mask must be", dict(mask=lambda x: x.double())),
+    (TypeError, "advantages must be", dict(adv=lambda x: x.half())),
+    (ValueError, "old_logp must have the shape", dict(old=lambda x: x.flatten())),
+    (ValueError, "temperature", dict(temperature=0.0)),
+    (ValueError, "kl_estimator", dict(kl_estimator="k4")),
+    (ValueError, "reduction", dict(reduction="none")),
+    (ValueError, "negative", dict(clip_param=-0.1)),
+    (ValueError, "finite", dict(entropy_coef=float("nan"))),
+    (ValueError, "needs ref_logp", dict(ref=lambda x: None)),
+]
+
+
+def refuse(device, error, text, change):
+    logits, tokens, old, adv, ref, mask = (x.to(device) for x in _case())
+    x = {"logits": logits, "tokens": tokens, "old": old, "adv": adv, "ref": ref, "mask": mask.float()}
+    kwargs = {"kl_coef": 0.1}
+    for key, value in change.items():
+        if key in x:
+            x[key] = value(x[key])
+        else:
+            kwargs[key] = value
+    with pytest.raises(error, match=text):
+        token_policy_loss_grad(x["logits"], x["tokens"], x["old"], x["adv"], ref_logp=x["ref"], mask=x["mask"], **kwargs)
+    with pytest.raises(error, match=text):
+        token_policy_loss(x["logits"], x["tokens"], x["old"], x["adv"], ref_logp=x["ref"], mask=x["mask"], **kwargs)
+
+
+@pytest.mark.parametrize("error,text,change", REFUSALS)
+def test_policy_refusals(error, text, change):
+    refuse("cpu", error, text, change)
+
+
+def refuse_preference(device):
+    logits, tokens, *_ = (x.to(device) for x in _case((4, 7)))
+    packed, flat = logits.flatten(0, 1), tokens.flatten()
+    off = torch.arange(0, 29, 7, device=device)
+    for error, text, args, kwargs in [
+        (ValueError, "even", (logits[:3], tokens[:3]), {}),
+        (ValueError, "offsets belong", (logits, tokens), {"offsets": off}),
+        (ValueError, "need the offsets", (packed, flat), {}),
+        (TypeError, "offsets must be", (packed, flat), {"offsets": off.float()}),
+        (ValueError, "offsets must be", (packed, flat), {"offsets": off[:, None]}),
+        (TypeError, "ref_logps must be", (logits, tokens, torch.zeros(4, device=device).double()), {}),
+        (ValueError, "ref_logps must be", (logits, tokens, torch.zeros(3, device=device)), {}),
+        (ValueError, "loss_type", (logits, tokens), {"loss_type": "dpo"}),
+        (ValueError, "beta", (logits, tokens), {"beta": 0.0}),
+        (ValueError, "label_smoothing", (logits, tokens), {"label_smoothing": 0.6}),
+        (ValueError, "belongs to", (logits, tokens), {"label_smoothing": 0.1, "loss_type": "ipo"}),
+    ]:
+        with pytest.raises(error, match=text):
+            preference_loss(*args, **kwargs)
+        with pytest.raises(error, match=text):
+            preference_loss_grad(*args, **kwargs)
+
+
+def test_preference_refusals():
+    refuse_preference("cpu")

@@ -101,4 +101,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   rlb_register_kernels(m);
   rlb_register_p2p(m);
   rlb_register_rnn(m);
+  rlb_register_token(m);
 }

@@ -14,6 +14,7 @@ from typing import Any
 
 import torch
 
+from ..ops.adamw import AdamW, AdamW8bit
 from .tensordict import TensorDict, is_tensordict
 
 
@@ -51,6 +52,9 @@ _OPTIMIZERS: dict[str, type] = {
     "adamw": torch.optim.AdamW,
     "sgd": torch.optim.SGD,
     "rmsprop": torch.optim.RMSprop,
+    # one step over every parameter at once, with 32-bit or 8-bit states (ops/adamw.py)
+    "adamw_fused": AdamW,
+    "adamw_8bit": AdamW8bit,
 }
 
 
