@@ -3,7 +3,8 @@
 The update is ``torch.optim.AdamW``'s (decoupled weight decay); the states of ``state_bits=32`` have its names and
 values. bfloat16 parameters are the upper half of a float32 weight whose lower 16 bits the optimizer keeps
 (``low_bits``), so a step is never lost to rounding: the pair is 4 bytes, the parameter alone is what the model reads.
-A parameter written from outside (a loaded checkpoint) is taken over by the next step, to within half of a bfloat16 step.
+A finite parameter written from outside (a loaded checkpoint) is taken over by the next step, to within half of a
+bfloat16 step.
 
 8-bit states hold, for each 256 consecutive elements of a tensor, a float32 scale and e4m3 codes: of the first moment
 and of the *root* of the second, whose range a code covers better. One step moves a moving average by far less than the
@@ -177,10 +178,10 @@ def _store_codes(x: torch.Tensor, rnd: torch.Tensor, codes: torch.Tensor, scales
 
 def _join(p: torch.Tensor, low: torch.Tensor) -> torch.Tensor:
     """The float32 weight of a bfloat16 one and its lower bits, unless those (of another weight) would carry it across
-    zero or past infinity."""
-    b, low = p.view(torch.int16).int() << 16, low.int()
-    w = b + low
-    return torch.where(((w ^ b) < 0) | ((low > 0) & p.isinf()), b, w).view(torch.float32)
+    zero."""
+    b = p.view(torch.int16).int() << 16
+    w = b + low.int()
+    return torch.where((w ^ b) < 0, b, w).view(torch.float32)
 
 
 def _step_torch(plans, settings, max_grad_norm):

@@ -19,12 +19,25 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// Kernel arguments hold at most 32,764 bytes: 400 tensors a launch; short lists travel in a small table.
+// Kernel arguments hold at most 32,764 bytes: 400 tensors a launch; short lists travel in a small table. The prepare
+// kernel's threads read `id` and nothing else: 64-byte entries read by 150 threads cost 20 us of constant-cache misses.
+struct Entry {
+  void *p, *g, *m, *v;
+  float *m_scale, *v_scale;
+  int16_t* low;
+  int64_t n;
+};
+
 template <int K>
 struct AdamTable {
   int count;
   uint32_t units;
-  AdamTensor t[K];
+  uint32_t run;               // consecutive units of a warp
+  uint32_t first_unit[K + 1];  // units before each tensor; the last entry: all of them
+  uint32_t vec[(K + 31) / 32];  // bit i: every pointer of tensor i allows 4-element accesses
+  uint16_t id[K];
+  Entry t[K];
+  __device__ __forceinline__ bool wide(int i) const { return vec[i >> 5] >> (i & 31) & 1u; }
 };
 
 // Per tensor, from its step count: 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), the step itself.
@@ -37,18 +50,30 @@ struct AdamConsts {
   double max_norm;
   float beta1, beta1c, beta2, beta2c, eps;
   int maximize;
+  uint32_t first_stream;
   uint64_t seed;
 };
 
-template <int K>
-__device__ __forceinline__ int find_tensor(const AdamTable<K>& t, uint32_t unit) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.t[mid].first_unit <= unit) lo = mid;
-    else hi = mid - 1;
+// Calls fn(tensor, first unit in the tensor, units) for a warp's units: runs of `run` consecutive units are dealt out over
+// all warps in turn, and a run is cut where a tensor ends. The tensor of a run's first unit is searched, the following
+// ones are found by stepping on.
+template <int K, typename Fn>
+__device__ __forceinline__ void walk_units(const AdamTable<K>& t, Fn&& fn) {
+  const uint32_t stride = gridDim.x * kWarps * t.run;
+  for (uint32_t at = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * t.run; at < t.units; at += stride) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (t.first_unit[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    const uint32_t end = min(at + t.run, t.units);
+    for (uint32_t unit = at; unit < end; ++lo) {  // an empty tensor ends where it begins
+      const uint32_t first = t.first_unit[lo], stop = min(end, t.first_unit[lo + 1]);
+      if (stop > unit) fn(lo, unit - first, stop - unit);
+      unit = max(unit, stop);
+    }
   }
-  return lo;
 }
 
 __device__ __forceinline__ double block_sum64(double x, double* smem) {  // result in every thread; fixed order
@@ -67,8 +92,8 @@ __device__ void prepare_factors(const AdamTable<K>& t, const AdamHyper& h, float
   double lr = h.lr;
   if (h.lr_device) lr = h.lr_f64 ? *static_cast<const double*>(h.lr_device) : *static_cast<const float*>(h.lr_device);
   for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
-    const float s = steps[t.t[i].id] + 1.f;
-    steps[t.t[i].id] = s;
+    const float s = steps[t.id[i]] + 1.f;
+    steps[t.id[i]] = s;
     f[i].decay = static_cast<float>(1.0 - lr * h.weight_decay);
     f[i].step_size = static_cast<float>(lr / (1.0 - pow(h.beta1, static_cast<double>(s))));
     f[i].unbias = static_cast<float>(1.0 / sqrt(1.0 - pow(h.beta2, static_cast<double>(s))));
@@ -98,6 +123,27 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
+// Sum of squares with its rounding errors: s + e is right to about 2^-45, so the norm in fp32 does not depend on the order
+// of the sum, at fp32 speed (summing in fp64 took 648 us for 335 M bf16 gradients, this 105: the conversions to fp64 run
+// at an eighth of the rate of fp32 arithmetic). T. J. Dekker, "A floating-point technique for extending the available
+// precision" (1971): the error of s + x is x - ((s + x) - s) where s is the larger; a sum of squares outgrows its terms.
+struct SquareSum {
+  float s = 0.f, e = 0.f;
+  template <bool kExact>  // kExact: x * x fits fp32 (bf16 gradients)
+  __device__ __forceinline__ void add(float x) {
+    const float q = __fmul_rn(x, x);
+    if (!kExact) e = __fadd_rn(e, __fmaf_rn(x, x, -q));
+    const float t = __fadd_rn(s, q);
+    e = __fadd_rn(e, __fsub_rn(q, __fsub_rn(t, s)));
+    s = t;
+  }
+  // s overflows (or holds a NaN): the errors are not numbers then, the sum is
+  __device__ __forceinline__ double value() const {
+    const double big = static_cast<double>(s);
+    return isfinite(s) ? big + static_cast<double>(e) : big;
+  }
+};
+
 // Sum of the squares of every gradient, one partial per block; the last block also prepares the factors.
 template <typename T, int K>
 __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_constant__ AdamTable<K> t,
@@ -108,65 +154,242 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
   __shared__ double smem[kWarps];
   if (blockIdx.x == gridDim.x - 1) prepare_factors(t, h, steps, f);
   const int lane = threadIdx.x & 31;
-  double sum = 0.0;
-  for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < t.units; unit += gridDim.x * kWarps) {
-    const AdamTensor& a = t.t[find_tensor(t, unit)];
-    const int64_t base = static_cast<int64_t>(unit - a.first_unit) * kAdamBlock;
+  constexpr bool kExact = sizeof(T) == 2;
+  constexpr int kBatch = kExact ? 4 : 2;  // units in flight: eight 8-byte or four 16-byte loads a lane
+  SquareSum sum[4];
+  walk_units(t, [&](int ti, uint32_t first, uint32_t units) {
+    const Entry& a = t.t[ti];
+    const int64_t base = static_cast<int64_t>(first) * kAdamBlock;
     const T* g = static_cast<const T*>(a.g) + base;
-    const int64_t left = a.n - base;
-    if (a.vec && left >= kAdamBlock) {
+    const int64_t left = min(a.n - base, static_cast<int64_t>(units) * kAdamBlock);
+    int64_t at = 0;
+    if (t.wide(ti)) {
+      for (; at + kBatch * kAdamBlock <= left; at += kBatch * kAdamBlock) {
+        float x[2 * kBatch][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float x[4];
-        load4(g + j * 128 + lane * 4, x);
+        for (int j = 0; j < 2 * kBatch; ++j) load4(g + at + j * 128 + lane * 4, x[j]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += static_cast<double>(x[e]) * static_cast<double>(x[e]);
+        for (int i = 0; i < 8 * kBatch; ++i) sum[i & 3].template add<kExact>(x[i >> 2][i & 3]);
       }
-    } else {
-      for (int64_t i = lane; i < left && i < kAdamBlock; i += 32) {
-        const double x = static_cast<double>(load1(g + i));
-        sum += x * x;
+      for (; at + 128 <= left; at += 128) {
+        float x[4];
+        load4(g + at + lane * 4, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i].template add<kExact>(x[i]);
       }
     }
-  }
-  sum = block_sum64(sum, smem);
-  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    for (at += lane; at < left; at += 32) sum[0].template add<kExact>(load1(g + at));
+  });
+  double total = sum[0].value() + sum[1].value() + (sum[2].value() + sum[3].value());
+  total = block_sum64(total, smem);
+  if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
 
 // ---- 8-bit codes ----------------------------------------------------------------------------------------------------
-// Value of an e4m3 code without sign (exact).
-__device__ __forceinline__ float e4m3_value(uint32_t code) {
-  return code >= 8u ? __uint_as_float((code << 20) + (120u << 23)) : static_cast<float>(code) * 0.001953125f;
+// An e4m3 number without sign is the upper 12 bits of the fp32 number 2^-120 times as large (subnormal ones included), so
+// codes and values differ by a shift and a product that is exact. Codes are handled where they leave those bits, in bits
+// 20 to 26, and four of them packed at the end.
+constexpr float kUp = 1.329227995784916e36f, kDown = 7.52316384526264e-37f;  // 2^120, 2^-120
+constexpr uint32_t kCode = 1u << 20;
+__device__ __forceinline__ float code_value(uint32_t bits) { return __uint_as_float(bits) * kUp; }
+// (rnd16 + 1 / 2) / 2^16 by its bits
+__device__ __forceinline__ float uniform(uint32_t rnd16) {
+  return __uint_as_float(0x3f800040u | rnd16 << 7) - 1.f;
 }
-// Code of the largest e4m3 value at most y, 0 <= y <= 448.
-__device__ __forceinline__ uint32_t e4m3_below(float y) {
-  return y >= 0.015625f ? (__float_as_uint(y) - (120u << 23)) >> 20 : static_cast<uint32_t>(y * 512.f);
+// The code below or above y (0 <= y <= 448, or half a unit more by the scale's rounding): above with probability
+// (y - below) / (above - below), which is what the 20 bits under the code say. Rounding the scaled y up leaves a fraction
+// that is not zero above every fraction below it.
+__device__ __forceinline__ uint32_t linear_code(float y, uint32_t rnd16) {
+  return __float_as_uint(__fmul_ru(y, kDown)) + (0xffff7u - 16u * rnd16);
+}
+// The same with probability (y^2 - below^2) / (above^2 - below^2).
+__device__ __forceinline__ uint32_t square_code(float y, uint32_t rnd16) {
+  const uint32_t below = __float_as_uint(__fmul_rz(y, kDown)) & 0xfff00000u;
+  const float lo = code_value(below), hi = code_value(below + kCode);
+  const bool up = __fmul_rn(__fmul_rn(hi - lo, hi + lo), uniform(rnd16)) < __fmul_rn(y - lo, y + lo);
+  return up ? below + kCode : below;
+}
+// Bytes 3 of four words.
+__device__ __forceinline__ uint32_t pack_top(const uint32_t (&x)[4]) {
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
+}
+__device__ __forceinline__ void unpack_codes(uint32_t c, float (&x)[4]) {  // signed values, exact
+  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c & 0xffffu), __NV_E4M3);
+  const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(c >> 16), __NV_E4M3);
+  const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 
-// The fp32 weight of a bf16 one and its lower bits. Lower bits that do not belong to the weight (it was written from
-// outside) move it by at most half of its last place, but across zero or past infinity they would make a NaN of it.
-__device__ __forceinline__ float join(float p, int32_t low) {
-  const uint32_t b = __float_as_uint(p), w = b + static_cast<uint32_t>(low);
-  const bool keep = static_cast<int32_t>(w ^ b) >= 0 && !(low > 0 && (b & 0x7fffffffu) == 0x7f800000u);
-  return __uint_as_float(keep ? w : b);
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-
-__device__ __forceinline__ float abs_max_bits(float a, float b) {  // NaN wins: its bits exceed every number's
-  return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
-}
-
-__device__ __forceinline__ uint32_t load_codes(const void* p) { return *static_cast<const uint32_t*>(p); }
 
 // ---- the step ---------------------------------------------------------------------------------------------------------
-// A warp takes a unit of 256 elements: lane l elements [4 l, 4 l + 4) and [128 + 4 l, ...), so every access of the warp
-// is contiguous. The unit is also the block of a scale, whose maximum is a warp reduction.
+// Four elements of every tensor of a step, as they lie in memory.
+template <typename T, bool kBits8>
+struct Quad {
+  float p[4], g[4], m[4], v[4];  // fp32 tensors
+  uint32_t pb[2], lb[2], gb[2];  // bf16 weights, their lower bits, gradients
+  uint32_t mc, vc;               // codes
+
+  static constexpr bool kSplit = sizeof(T) == 2;
+
+  __device__ __forceinline__ void load(const Entry& a, int64_t at) {
+    if (kSplit) {
+      const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.p) + at);
+      const uint2 y = *reinterpret_cast<const uint2*>(a.low + at);
+      const uint2 z = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.g) + at);
+      pb[0] = x.x, pb[1] = x.y, lb[0] = y.x, lb[1] = y.y, gb[0] = z.x, gb[1] = z.y;
+    } else {
+      load4(static_cast<const float*>(a.p) + at, p);
+      load4(static_cast<const float*>(a.g) + at, g);
+    }
+    if (kBits8) {
+      mc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + at);
+      vc = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + at);
+    } else {
+      load4(static_cast<const float*>(a.m) + at, m);
+      load4(static_cast<const float*>(a.v) + at, v);
+    }
+  }
+  __device__ __forceinline__ void store(const Entry& a, int64_t at) const {
+    if (kSplit) {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.p) + at) = make_uint2(pb[0], pb[1]);
+      *reinterpret_cast<uint2*>(a.low + at) = make_uint2(lb[0], lb[1]);
+    } else {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.p) + at) = make_float4(p[0], p[1], p[2], p[3]);
+    }
+    if (kBits8) {
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + at) = mc;
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + at) = vc;
+    } else {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.m) + at) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(static_cast<float*>(a.v) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+  // The same for the `in` first elements, one by one; the others count as zeros.
+  __device__ __forceinline__ void load_some(const Entry& a, int64_t at, int in) {
+    pb[0] = pb[1] = lb[0] = lb[1] = gb[0] = gb[1] = mc = vc = 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      p[e] = g[e] = m[e] = v[e] = 0.f;
+      if (e >= in) continue;
+      if (kSplit) {
+        pb[e >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(a.p)[at + e]) << (16 * (e & 1));
+        lb[e >> 1] |= static_cast<uint32_t>(static_cast<uint16_t>(a.low[at + e])) << (16 * (e & 1));
+        gb[e >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(a.g)[at + e]) << (16 * (e & 1));
+      } else {
+        p[e] = static_cast<const float*>(a.p)[at + e];
+        g[e] = static_cast<const float*>(a.g)[at + e];
+      }
+      if (kBits8) {
+        mc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.m)[at + e]) << (8 * e);
+        vc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.v)[at + e]) << (8 * e);
+      } else {
+        m[e] = static_cast<const float*>(a.m)[at + e];
+        v[e] = static_cast<const float*>(a.v)[at + e];
+      }
+    }
+  }
+  __device__ __forceinline__ void store_some(const Entry& a, int64_t at, int in) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= in) continue;
+      if (kSplit) {
+        static_cast<uint16_t*>(a.p)[at + e] = static_cast<uint16_t>(pb[e >> 1] >> (16 * (e & 1)));
+        a.low[at + e] = static_cast<int16_t>(lb[e >> 1] >> (16 * (e & 1)));
+      } else {
+        static_cast<float*>(a.p)[at + e] = p[e];
+      }
+      if (kBits8) {
+        static_cast<uint8_t*>(a.m)[at + e] = static_cast<uint8_t>(mc >> (8 * e));
+        static_cast<uint8_t*>(a.v)[at + e] = static_cast<uint8_t>(vc >> (8 * e));
+      } else {
+        static_cast<float*>(a.m)[at + e] = m[e];
+        static_cast<float*>(a.v)[at + e] = v[e];
+      }
+    }
+  }
+
+  // Memory's form to fp32 and back. Rounding a weight to bf16 by adding half a unit (halves up) leaves a remainder of 16
+  // signed bits, which are the fp32 weight's lower 16 bits as they are.
+  __device__ __forceinline__ void decode(float m_scale, float v_scale) {
+    if (kSplit) {
+      uint32_t odd = 0u;  // a sign that the lower bits have changed: they belong to another weight
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t b = e & 1 ? pb[e >> 1] & 0xffff0000u : pb[e >> 1] << 16;
+        const uint32_t joined = __byte_perm(lb[e >> 1], pb[e >> 1], e & 1 ? 0x7632 : 0x5410);
+        const uint32_t w = joined - ((joined & 0x8000u) << 1);
+        odd |= w ^ b;
+        p[e] = __uint_as_float(w);
+        g[e] = __uint_as_float(e & 1 ? gb[e >> 1] & 0xffff0000u : gb[e >> 1] << 16);
+      }
+      if (static_cast<int32_t>(odd) < 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t b = e & 1 ? pb[e >> 1] & 0xffff0000u : pb[e >> 1] << 16;
+          if (static_cast<int32_t>(__float_as_uint(p[e]) ^ b) < 0) p[e] = __uint_as_float(b);
+        }
+      }
+    }
+    if (kBits8) {
+      unpack_codes(mc, m);
+      unpack_codes(vc, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = __fmul_rn(m[e], m_scale);
+        const float r = __fmul_rn(v[e], v_scale);
+        v[e] = __fmul_rn(r, r);
+      }
+    }
+  }
+  __device__ __forceinline__ void encode_weights() {
+    if (!kSplit) return;
+    uint32_t b[4];
+    float finite = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      finite = fmaf(p[e], 0.f, finite);
+      b[e] = __float_as_uint(p[e]);
+    }
+    if (isnan(finite)) {  // a NaN's bits do not survive the carry: one that does
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = isnan(p[e]) ? 0x7fc00000u : b[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      pb[i] = __byte_perm(b[2 * i] + 0x8000u, b[2 * i + 1] + 0x8000u, 0x7632);
+      lb[i] = __byte_perm(b[2 * i], b[2 * i + 1], 0x5410);
+    }
+  }
+  // `v` holds the roots.
+  __device__ __forceinline__ void encode_states(float m_inv, float v_inv, const Philox& rnd) {
+    uint32_t x[4], y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // the stored m is right on average
+      const uint32_t c = linear_code(__fmul_rn(fabsf(m[e]), m_inv), rnd.c[e] & 0xffffu);
+      x[e] = (c << 4 & 0x7f000000u) | (__float_as_uint(m[e]) & 0x80000000u);
+      // v, not its root, is right on average; never down to zero, which would leave m / eps as the next step
+      const uint32_t d = square_code(__fmul_rn(v[e], v_inv), rnd.c[e] >> 16);
+      y[e] = (v_inv > 0.f && v[e] > 0.f ? max(d, kCode) : d) << 4 & 0x7f000000u;
+    }
+    mc = pack_top(x);
+    vc = pack_top(y);
+  }
+};
+
+// A warp takes units of 256 elements: lane l elements [4 l, 4 l + 4) and [128 + 4 l, ...), so every access of the warp is
+// contiguous. The unit is also the block of a scale, whose maximum is a warp reduction.
 template <typename T, bool kBits8, int K>
-__global__ void __launch_bounds__(kThreads) adamw_step_kernel(const __grid_constant__ AdamTable<K> t,
+__global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_constant__ AdamTable<K> t,
                                                               const AdamConsts c, const AdamFactors* factors,
                                                               const double* partial, int partials, float* norm_out) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
-  constexpr bool kSplit = sizeof(T) == 2;  // bf16 weights with their lower bits
   __shared__ double smem[kWarps];
   float clip = 1.f;
   if (partials > 0) {
@@ -179,187 +402,75 @@ __global__ void __launch_bounds__(kThreads) adamw_step_kernel(const __grid_const
   }
   if (c.maximize) clip = -clip;
   const int lane = threadIdx.x & 31;
-  for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < t.units; unit += gridDim.x * kWarps) {
-    const int ti = find_tensor(t, unit);
-    const AdamTensor& a = t.t[ti];
-    const int64_t base = static_cast<int64_t>(unit - a.first_unit) * kAdamBlock;
-    const int left = static_cast<int>(min(a.n - base, static_cast<int64_t>(kAdamBlock)));
-    const bool vec = a.vec && left == kAdamBlock;
-    T* P = static_cast<T*>(a.p) + base;
-    const T* G = static_cast<const T*>(a.g) + base;
-    float p[8], g[8], m[8], v[8];
-    uint32_t mc[2], vc[2];
-    const int64_t blk = base / kAdamBlock;
+  walk_units(t, [&](int ti, uint32_t first, uint32_t units) {
+    const Entry a = t.t[ti];
+    const AdamFactors f = factors[ti];
+    const bool wide = t.wide(ti);
+    for (uint32_t u = first; u < first + units; ++u) {
+      const int64_t at = static_cast<int64_t>(u) * kAdamBlock + lane * 4;
+      const int left = static_cast<int>(min(a.n - static_cast<int64_t>(u) * kAdamBlock, static_cast<int64_t>(kAdamBlock)));
+      const bool whole = wide && left == kAdamBlock;
+      Quad<T, kBits8> q[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int o = j * 128 + lane * 4;
-      float(&pj)[4] = *reinterpret_cast<float(*)[4]>(p + 4 * j);
-      float(&gj)[4] = *reinterpret_cast<float(*)[4]>(g + 4 * j);
-      float(&mj)[4] = *reinterpret_cast<float(*)[4]>(m + 4 * j);
-      float(&vj)[4] = *reinterpret_cast<float(*)[4]>(v + 4 * j);
-      if (vec) {
-        load4(P + o, pj);
-        load4(G + o, gj);
-        if (kSplit) {
-          const uint2 w = *reinterpret_cast<const uint2*>(a.low + base + o);
-          pj[0] = join(pj[0], static_cast<int16_t>(w.x & 0xffffu));
-          pj[1] = join(pj[1], (static_cast<int32_t>(w.x) >> 16));
-          pj[2] = join(pj[2], static_cast<int16_t>(w.y & 0xffffu));
-          pj[3] = join(pj[3], (static_cast<int32_t>(w.y) >> 16));
-        }
-        if (kBits8) {
-          mc[j] = load_codes(static_cast<uint8_t*>(a.m) + base + o);
-          vc[j] = load_codes(static_cast<uint8_t*>(a.v) + base + o);
-        } else {
-          load4(static_cast<float*>(a.m) + base + o, mj);
-          load4(static_cast<float*>(a.v) + base + o, vj);
-        }
-      } else {
-        mc[j] = vc[j] = 0u;
+      for (int j = 0; j < 2; ++j) {
+        if (whole) q[j].load(a, at + j * 128);
+        else q[j].load_some(a, at + j * 128, left - j * 128 - lane * 4);
+      }
+      const float ms = kBits8 ? a.m_scale[u] : 0.f, vs = kBits8 ? a.v_scale[u] : 0.f;
+      float m_top = 0.f, r_top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        q[j].decode(ms, vs);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool in = o + e < left;
-          pj[e] = in ? load1(P + o + e) : 0.f;
-          gj[e] = in ? load1(G + o + e) : 0.f;
-          if (kSplit && in) pj[e] = join(pj[e], a.low[base + o + e]);
+          float &p = q[j].p[e], &m = q[j].m[e], &v = q[j].v[e];
+          const float g = __fmul_rn(q[j].g[e], clip);
+          m = __fadd_rn(__fmul_rn(m, c.beta1), __fmul_rn(g, c.beta1c));
+          v = __fadd_rn(__fmul_rn(v, c.beta2), __fmul_rn(__fmul_rn(g, g), c.beta2c));
+          const float r = __fsqrt_rn(v);
+          const float x = __fdiv_rn(m, __fadd_rn(__fmul_rn(r, f.unbias), c.eps));
+          p = __fsub_rn(__fmul_rn(p, f.decay), __fmul_rn(f.step_size, x));
           if (kBits8) {
-            if (in) {
-              mc[j] |= static_cast<uint32_t>(static_cast<uint8_t*>(a.m)[base + o + e]) << (8 * e);
-              vc[j] |= static_cast<uint32_t>(static_cast<uint8_t*>(a.v)[base + o + e]) << (8 * e);
-            }
-          } else {
-            mj[e] = in ? static_cast<float*>(a.m)[base + o + e] : 0.f;
-            vj[e] = in ? static_cast<float*>(a.v)[base + o + e] : 0.f;
+            v = r;
+            m_top = max_nan(m_top, fabsf(m));
+            r_top = max_nan(r_top, r);
           }
         }
       }
-    }
-    if (kBits8) {
-      const float ms = a.m_scale[blk], vs = a.v_scale[blk];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t cm = mc[i >> 2] >> (8 * (i & 3)), cv = vc[i >> 2] >> (8 * (i & 3));
-        const float mv = e4m3_value(cm & 0x7fu);
-        m[i] = __fmul_rn(cm & 0x80u ? -mv : mv, ms);
-        const float r = __fmul_rn(e4m3_value(cv & 0x7fu), vs);
-        v[i] = __fmul_rn(r, r);
-      }
-    }
-    const AdamFactors f = factors[ti];
-    float m_top = 0.f, r_top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gi = __fmul_rn(g[i], clip);
-      m[i] = __fadd_rn(__fmul_rn(m[i], c.beta1), __fmul_rn(gi, c.beta1c));
-      v[i] = __fadd_rn(__fmul_rn(v[i], c.beta2), __fmul_rn(__fmul_rn(gi, gi), c.beta2c));
-      const float r = __fsqrt_rn(v[i]);
-      const float u = __fdiv_rn(m[i], __fadd_rn(__fmul_rn(r, f.unbias), c.eps));
-      p[i] = __fsub_rn(__fmul_rn(p[i], f.decay), __fmul_rn(f.step_size, u));
       if (kBits8) {
-        v[i] = r;
-        m_top = abs_max_bits(m_top, m[i]);
-        r_top = abs_max_bits(r_top, r);
-      }
-    }
-    if (kBits8) {
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) {
-        m_top = abs_max_bits(m_top, __shfl_xor_sync(0xffffffffu, m_top, o));
-        r_top = abs_max_bits(r_top, __shfl_xor_sync(0xffffffffu, r_top, o));
-      }
-      // blocks below 1e-30 are held as zero, so the scale's inverse stays finite
-      const bool m_on = !(m_top < 1e-30f), r_on = !(r_top < 1e-30f);
-      const float mi = m_on ? __fmul_rn(__frcp_rn(m_top), 448.f) : 0.f;
-      const float ri = r_on ? __fmul_rn(__frcp_rn(r_top), 448.f) : 0.f;
-      if (lane == 0) {
-        a.m_scale[blk] = m_on ? __fmul_rn(m_top, 1.f / 448.f) : 0.f;
-        a.v_scale[blk] = r_on ? __fmul_rn(r_top, 1.f / 448.f) : 0.f;
+        for (int o = 16; o >= 1; o >>= 1) {
+          m_top = max_nan(m_top, __shfl_xor_sync(0xffffffffu, m_top, o));
+          r_top = max_nan(r_top, __shfl_xor_sync(0xffffffffu, r_top, o));
+        }
+        // blocks below 1e-30 are held as zero, so the scale's inverse stays finite
+        const bool m_on = !(m_top < 1e-30f), r_on = !(r_top < 1e-30f);
+        const float mi = m_on ? __fmul_rn(__frcp_rn(m_top), 448.f) : 0.f;
+        const float ri = r_on ? __fmul_rn(__frcp_rn(r_top), 448.f) : 0.f;
+        if (lane == 0) {
+          a.m_scale[u] = m_on ? __fmul_rn(m_top, 1.f / 448.f) : 0.f;
+          a.v_scale[u] = r_on ? __fmul_rn(r_top, 1.f / 448.f) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint64_t i4 = static_cast<uint64_t>(at + j * 128) >> 2;
+          q[j].encode_states(mi, ri, philox10(static_cast<uint32_t>(i4), static_cast<uint32_t>(i4 >> 32),
+                                              c.first_stream + t.id[ti], f.step, static_cast<uint32_t>(c.seed),
+                                              static_cast<uint32_t>(c.seed >> 32)));
+        }
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint64_t idx4 = static_cast<uint64_t>(base + j * 128 + lane * 4) >> 2;
-        const Philox rnd = philox10(static_cast<uint32_t>(idx4), static_cast<uint32_t>(idx4 >> 32), a.stream, f.step,
-                                    static_cast<uint32_t>(c.seed), static_cast<uint32_t>(c.seed >> 32));
-        mc[j] = vc[j] = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * j + e;
-          // m: up with probability (y - low) / (high - low), so the stored value is right on average
-          float u = __fmul_rn(static_cast<float>(rnd.c[e] & 0xffffu) + 0.5f, 1.f / 65536.f);
-          float y = fminf(__fmul_rn(fabsf(m[i]), mi), 448.f);
-          uint32_t code = e4m3_below(y);
-          float lo = e4m3_value(code), hi = e4m3_value(code + 1u);
-          if (__fmul_rn(hi - lo, u) < y - lo) ++code;
-          mc[j] |= (code | (m[i] < 0.f ? 0x80u : 0u)) << (8 * e);
-          // sqrt(v): up with probability (y^2 - low^2) / (high^2 - low^2), so that v, not its root, is right on average;
-          // never down to zero, which would leave m / eps as the next step
-          u = __fmul_rn(static_cast<float>(rnd.c[e] >> 16) + 0.5f, 1.f / 65536.f);
-          y = fminf(__fmul_rn(v[i], ri), 448.f);
-          code = e4m3_below(y);
-          lo = e4m3_value(code), hi = e4m3_value(code + 1u);
-          if (__fmul_rn(__fmul_rn(hi - lo, hi + lo), u) < __fmul_rn(y - lo, y + lo)) ++code;
-          if (r_on && v[i] > 0.f) code = max(code, 1u);
-          vc[j] |= code << (8 * e);
-        }
+        q[j].encode_weights();
+        if (whole) q[j].store(a, at + j * 128);
+        else q[j].store_some(a, at + j * 128, left - j * 128 - lane * 4);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int o = j * 128 + lane * 4;
-      uint32_t hi[4];
-      int32_t lo[4];
-      if (kSplit) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // round to nearest, halves up: the remainder fits 16 signed bits
-          const uint32_t b = __float_as_uint(p[4 * j + e]);
-          const bool nan = (b & 0x7fffffffu) > 0x7f800000u;
-          hi[e] = nan ? 0x7fc0u : (b + 0x8000u) >> 16;
-          lo[e] = nan ? 0 : static_cast<int32_t>(b - (hi[e] << 16));
-        }
-      }
-      if (vec) {
-        if (kSplit) {
-          *reinterpret_cast<uint2*>(P + o) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
-          *reinterpret_cast<uint2*>(a.low + base + o) =
-              make_uint2((lo[0] & 0xffffu) | static_cast<uint32_t>(lo[1]) << 16,
-                         (lo[2] & 0xffffu) | static_cast<uint32_t>(lo[3]) << 16);
-        } else {
-          *reinterpret_cast<float4*>(P + o) = make_float4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
-        }
-        if (kBits8) {
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + base + o) = mc[j];
-          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + base + o) = vc[j];
-        } else {
-          *reinterpret_cast<float4*>(static_cast<float*>(a.m) + base + o) =
-              make_float4(m[4 * j], m[4 * j + 1], m[4 * j + 2], m[4 * j + 3]);
-          *reinterpret_cast<float4*>(static_cast<float*>(a.v) + base + o) =
-              make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (o + e >= left) continue;
-          if (kSplit) {
-            reinterpret_cast<uint16_t*>(P)[o + e] = static_cast<uint16_t>(hi[e]);
-            a.low[base + o + e] = static_cast<int16_t>(lo[e]);
-          } else {
-            reinterpret_cast<float*>(P)[o + e] = p[4 * j + e];
-          }
-          if (kBits8) {
-            static_cast<uint8_t*>(a.m)[base + o + e] = static_cast<uint8_t>(mc[j] >> (8 * e));
-            static_cast<uint8_t*>(a.v)[base + o + e] = static_cast<uint8_t>(vc[j] >> (8 * e));
-          } else {
-            static_cast<float*>(a.m)[base + o + e] = m[4 * j + e];
-            static_cast<float*>(a.v)[base + o + e] = v[4 * j + e];
-          }
-        }
-      }
-    }
-  }
+  });
 }
 
 constexpr int kSmallTable = 40, kLargeTable = 400;
-constexpr int kNormBlocks = 592;
+constexpr int kNormBlocks = 1184;
 static_assert(sizeof(AdamTable<kLargeTable>) + 256 <= 32764, "kernel arguments");
 
 int sm_count() {
@@ -373,20 +484,28 @@ template <int K>
 void fill_table(AdamTable<K>& t, const AdamLaunch& a, int first) {
   t.count = std::min(K, a.count - first);
   t.units = 0;
+  for (uint32_t& x : t.vec) x = 0;
   for (int i = 0; i < t.count; ++i) {
-    AdamTensor& x = t.t[i] = a.tensors[first + i];
-    x.first_unit = t.units;
+    const AdamTensor& x = a.tensors[first + i];
+    t.t[i] = Entry{x.p, x.g, x.m, x.v, x.m_scale, x.v_scale, x.low, x.n};
+    t.id[i] = static_cast<uint16_t>(x.id);
+    t.first_unit[i] = t.units;
     t.units += static_cast<uint32_t>((x.n + kAdamBlock - 1) / kAdamBlock);
     const uintptr_t wide = a.bf16 ? 7u : 15u, state = a.bits8 ? 3u : 15u;
     const uintptr_t bad = ((reinterpret_cast<uintptr_t>(x.p) | reinterpret_cast<uintptr_t>(x.g) |
                             reinterpret_cast<uintptr_t>(x.low)) & wide) |
                           ((reinterpret_cast<uintptr_t>(x.m) | reinterpret_cast<uintptr_t>(x.v)) & state);
-    x.vec = bad == 0;
+    if (bad == 0) t.vec[i >> 5] |= 1u << (i & 31);
   }
+  t.first_unit[t.count] = t.units;
+  // up to 8 units a run, while every warp of a full grid still has one
+  t.run = std::min<uint32_t>(8, std::max<uint32_t>(1, t.units / (148 * 6 * kWarps)));
 }
 
-unsigned norm_blocks(uint32_t units) {
-  return static_cast<unsigned>(std::min<uint32_t>(kNormBlocks, std::max<uint32_t>(1, (units + kWarps - 1) / kWarps)));
+// Blocks whose warps all have a run.
+unsigned blocks_of(uint32_t units, uint32_t run, unsigned most) {
+  const uint32_t runs = (units + run - 1) / run;
+  return std::min<unsigned>(most, std::max<unsigned>(1, (runs + kWarps - 1) / kWarps));
 }
 
 // What one step over several lists shares: the partial sums of the norm come from every list before the first is stepped.
@@ -405,7 +524,7 @@ cudaError_t prepare(const AdamLaunch& a, AdamFactors* factors, Shared& sh, cudaS
     fill_table(t, a, first);
     cudaError_t e;
     if (sh.max_norm > 0.0) {
-      const unsigned grid = norm_blocks(t.units);
+      const unsigned grid = blocks_of(t.units, t.run, kNormBlocks);
       e = launch_pdl(adamw_norm_kernel<T, K>, dim3(grid), dim3(kThreads), 0, stream, t, a.h, a.steps, factors + first,
                      sh.partial + sh.partials);
       sh.partials += static_cast<int>(grid);
@@ -423,12 +542,11 @@ cudaError_t step(const AdamLaunch& a, const AdamFactors* factors, Shared& sh, cu
   c.beta1 = static_cast<float>(a.h.beta1), c.beta1c = static_cast<float>(1.0 - a.h.beta1);
   c.beta2 = static_cast<float>(a.h.beta2), c.beta2c = static_cast<float>(1.0 - a.h.beta2);
   c.eps = static_cast<float>(a.h.eps), c.max_norm = sh.max_norm;
-  c.maximize = a.h.maximize, c.seed = a.h.seed;
+  c.maximize = a.h.maximize, c.seed = a.h.seed, c.first_stream = a.first_stream;
   AdamTable<K> t;
   for (int first = 0; first < a.count; first += K) {
     fill_table(t, a, first);
-    const unsigned blocks = std::max<unsigned>(1, (t.units + kWarps - 1) / kWarps);  // an empty list writes the norm
-    const unsigned grid = std::min<unsigned>(static_cast<unsigned>(sm_count()) * 6, blocks);
+    const unsigned grid = blocks_of(t.units, t.run, static_cast<unsigned>(sm_count()) * 6);  // one at least: the norm
     const cudaError_t e = launch_pdl(adamw_step_kernel<T, kBits8, K>, dim3(grid), dim3(kThreads), 0, stream, t, c,
                                      factors + first, static_cast<const double*>(sh.partial), sh.partials, sh.norm);
     sh.norm = nullptr;  // written once

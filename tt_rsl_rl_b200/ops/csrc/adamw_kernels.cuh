@@ -20,10 +20,7 @@ struct AdamTensor {
   float *m_scale, *v_scale;
   int16_t* low;             // bf16 weights: the fp32 weight's lower bits
   int64_t n;
-  uint32_t first_unit;      // units of kAdamBlock elements before this tensor (filled by the launcher)
-  uint32_t id;              // the tensor's place in `steps`
-  uint32_t stream;          // the tensor's stream of random numbers
-  uint32_t vec;             // 1: every pointer allows 4-element accesses (filled by the launcher)
+  uint32_t id;              // the tensor's place in `steps`, below 65,536
 };
 
 struct AdamHyper {
@@ -39,6 +36,7 @@ struct AdamLaunch {
   int count;
   int bf16, bits8;
   AdamHyper h;
+  uint32_t first_stream;  // tensor `id` draws its random numbers from stream first_stream + id
   float* steps;        // [tensors of the plan] steps taken; advanced by one for the tensors of this launch
 };
 // One step of several lists of tensors. max_norm > 0: every gradient is scaled by min(1, max_norm / (norm + 1e-6)) with

@@ -72,6 +72,13 @@ struct Logits {
                       text(t.sizes().slice(0, t.dim() - 1)), ", got ", text(x.sizes()));
     return x.contiguous();
   }
+  // Whether every row of a gradient starts at the same place within 16 bytes as its logits.
+  bool same_phase(const Tensor& grad) const {
+    const int64_t size = t.element_size();
+    auto same = [&](int64_t x, int64_t y) { return (x - y) * size % 16 == 0; };
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) - reinterpret_cast<uintptr_t>(grad.data_ptr())) % 16 == 0 &&
+           same(t.stride(-2), grad.stride(-2)) && (t.dim() == 2 || same(t.stride(0), grad.stride(0)));
+  }
   // Where rows start at different places within 16 bytes, the gradient takes the logits' strides (if that costs at most
   // a quarter more memory), so that both can be accessed 16 bytes at a time.
   Tensor gradient() const {
@@ -194,33 +201,43 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   q.kl_coef = static_cast<float>(kl_coef), q.entropy_coef = static_cast<float>(entropy_coef);
   q.kl_kind = static_cast<int>(kl_kind);
   Tensor out = torch::empty({6}, l.f32()), logp = torch::empty(l.lead(), l.f32());
-  Tensor entropy = torch::empty(l.lead(), l.f32()), ml = torch::empty({l.rows, 2}, l.f32());
-  Tensor terms = torch::empty({l.rows, 4}, l.f32()), coef = torch::empty({l.rows, 2}, l.f32());
+  Tensor terms = torch::empty({l.rows, 4}, l.f32()), entropy, ml, coef, grad;
+  if (want_grad) grad = l.gradient();
+  const bool one_pass = want_grad && l.same_phase(grad);
   rlb::TokenStatsArgs a{};
   a.dtype = l.dtype, a.rows = l.rows, a.vocab = l.vocab, a.z = l.z, a.idx = ix.idx, a.inv_temp = inverse(temperature);
   a.logp = logp.data_ptr<float>();
-  a.entropy = entropy.data_ptr<float>();
-  a.ml = reinterpret_cast<float2*>(ml.data_ptr<float>());
   a.policy = &q;
   a.terms = reinterpret_cast<float4*>(terms.data_ptr<float>());
-  a.coef = reinterpret_cast<float2*>(coef.data_ptr<float>());
-  ok(rlb::token_stats(a, stream), "token_policy_loss");
+  const float* scale_device = scale_ptr(l, grad_scale_device);
+  if (one_pass) {
+    ok(rlb::token_policy(a, Logits::rows_of(grad), static_cast<float>(grad_scale), scale_device, mean, stream),
+       "token_policy_loss");
+  } else {
+    entropy = torch::empty(l.lead(), l.f32()), ml = torch::empty({l.rows, 2}, l.f32());
+    coef = torch::empty({l.rows, 2}, l.f32());
+    a.entropy = entropy.data_ptr<float>();
+    a.ml = reinterpret_cast<float2*>(ml.data_ptr<float>());
+    a.coef = reinterpret_cast<float2*>(coef.data_ptr<float>());
+    ok(rlb::token_stats(a, stream), "token_policy_loss");
+  }
   rlb::PolicyFinishArgs f{};
   f.rows = l.rows, f.terms = a.terms, f.idx = ix.idx, f.vocab = l.vocab, f.kl_coef = q.kl_coef;
   f.entropy_coef = q.entropy_coef, f.mean = mean, f.out = out.data_ptr<float>();
   ok(rlb::policy_finish(f, stream), "token_policy_loss");
   if (!want_grad) return {out, logp, entropy, ml, coef};
-  Tensor grad = l.gradient();
-  rlb::TokenGradArgs g{};
-  g.dtype = l.dtype, g.rows = l.rows, g.vocab = l.vocab, g.z = l.z, g.idx = ix.idx, g.inv_temp = a.inv_temp;
-  g.out = Logits::rows_of(grad);
-  g.ml = a.ml, g.entropy = a.entropy;
-  g.a = coef.data_ptr<float>(), g.a_stride = 2;
-  if (q.entropy_coef != 0.f) g.b = coef.data_ptr<float>() + 1, g.b_stride = 2;
-  g.weighted = 1;
-  g.scale = static_cast<float>(grad_scale), g.scale_a = scale_ptr(l, grad_scale_device);
-  g.scale_b = out.data_ptr<float>() + 5;
-  ok(rlb::token_grad(g, stream), "token_policy_loss");
+  if (!one_pass) {
+    rlb::TokenGradArgs g{};
+    g.dtype = l.dtype, g.rows = l.rows, g.vocab = l.vocab, g.z = l.z, g.idx = ix.idx, g.inv_temp = a.inv_temp;
+    g.out = Logits::rows_of(grad);
+    g.ml = a.ml, g.entropy = a.entropy;
+    g.a = coef.data_ptr<float>(), g.a_stride = 2;
+    if (q.entropy_coef != 0.f) g.b = coef.data_ptr<float>() + 1, g.b_stride = 2;
+    g.weighted = 1;
+    g.scale = static_cast<float>(grad_scale), g.scale_a = scale_device;
+    g.scale_b = out.data_ptr<float>() + 5;
+    ok(rlb::token_grad(g, stream), "token_policy_loss");
+  }
   return {out, logp, grad};
 }
 
@@ -323,6 +340,7 @@ class AdamWPlan {
         low_(std::move(low)), steps_(std::move(steps)), first_stream_(first_stream) {
     const size_t n = p_.size();
     TORCH_CHECK_VALUE(n > 0, "AdamWPlan: no parameters");
+    TORCH_CHECK_VALUE(n < 65536, "AdamWPlan: at most 65,535 parameters");
     TORCH_CHECK_VALUE(m_.size() == n && v_.size() == n, "AdamWPlan: one exp_avg and one exp_avg_sq per parameter");
     const auto dt = p_[0].scalar_type();
     TORCH_CHECK_TYPE(dt == torch::kFloat32 || dt == torch::kBFloat16,
@@ -387,13 +405,13 @@ class AdamWPlan {
       if (bf16_) t.low = low_[i].data_ptr<int16_t>();
       t.n = p.numel();
       t.id = static_cast<uint32_t>(i);
-      t.stream = static_cast<uint32_t>(first_stream_ + static_cast<int64_t>(i));
       table_.push_back(t);
     }
     rlb::AdamLaunch a{};
     a.tensors = table_.data(), a.count = static_cast<int>(table_.size());
     a.bf16 = bf16_, a.bits8 = bits8_;
     a.steps = steps_.data_ptr<float>();
+    a.first_stream = static_cast<uint32_t>(first_stream_);
     return a;
   }
 

@@ -18,11 +18,17 @@ namespace cg = cooperative_groups;
 
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kFar = -1e30f;  // stands for the exponent of a column of probability zero in products that must stay finite
+constexpr float kFar = -1e30f;  // exponent of a column of probability zero: its product with that zero stays a number
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float at_least_far(float d) {  // a NaN stays one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(d), "f"(kFar));
   return y;
 }
 
@@ -31,6 +37,10 @@ struct Elem;
 template <>
 struct Elem<float> {
   static constexpr int kPerVec = 4;
+  static constexpr uint32_t kNone = 0xff800000u;  // -inf
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
   static __device__ __forceinline__ float get(float x) { return x; }
   static __device__ __forceinline__ float put(float x) { return x; }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
@@ -43,6 +53,12 @@ struct Elem<float> {
 template <>
 struct Elem<__nv_bfloat16> {
   static constexpr int kPerVec = 8;
+  static constexpr uint32_t kNone = 0xff80ff80u;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
@@ -61,6 +77,12 @@ struct Elem<__nv_bfloat16> {
 template <>
 struct Elem<__half> {
   static constexpr int kPerVec = 8;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
   static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
@@ -105,68 +127,119 @@ __device__ __forceinline__ int64_t row_token(const TokenIndex& t, int64_t row, i
 }
 
 // ---- running softmax ------------------------------------------------------------------------------------------------
+// The exponent of a column is d = z hi + c, one fused multiply-add, with c = -m hi for the largest z so far: any c near
+// -m hi serves as long as the sums and their use agree on it. `hi` is log2(e) / T rounded to a float; what it lacks (lo)
+// shifts every exponent of a row the same way, an error that the sum over a sequence's rows would add up, so the end
+// corrects for it: d ln s / dk = sum p z.
+//
 // m: maximum so far (starts at the lowest finite value, so rows and columns at that value or at -inf stay defined),
-// s: sum of 2^((z - m) k), t: sum of 2^((z - m) k) (z - m) k (entropy only).
+// s: sum of 2^d, t: sum of 2^d d.
 struct Soft {
   float m, s, t;
 };
 
-// log2(e) / T as a sum of two floats, the first rounded towards zero: with one float its rounding shifts every exponent
-// the same way, an error of the log-sum that all rows share and that the sum over a sequence adds up (mean error of a
-// log-probability over 2,000 rows of 65,536 columns: below 1e-8; with one float, and rescaling by ex2.approx, 9e-8).
 struct Base {
-  float hi, lo;  // both positive, so -inf stays -inf
-  float inv_temp;
-  __device__ __forceinline__ float operator()(float dz) const { return fmaf(dz, hi, dz * lo); }
-  // Factor of sums whose maximum grows, dz = old - new: rare, so by the accurate function.
-  __device__ __forceinline__ float fall(float dz) const { return expf(dz * inv_temp); }
+  float hi, lo;         // log2(e) / T as a sum
+  float inv, inv_lack;  // 1 / T as a sum
 };
 
-template <bool kEnt>
+constexpr float kLow = -1e30f;  // below this maximum c overflows; such rows (only lowest values) subtract first
+
+__device__ __forceinline__ float shift_of(float m, const Base& k) { return -m * k.hi; }
+
+// Rare, so by the accurate function: a chain of these with ex2.approx, which is low by 5e-8 on average, shows in sums.
 __device__ __forceinline__ void soft_raise(Soft& a, float m, const Base& k) {
-  const float c = k.fall(a.m - m);
-  if (kEnt) a.t = c * fmaf(a.s, fmaxf(k(a.m - m), kFar), a.t);
-  a.s *= c;
+  const float d = m > kLow && a.m > kLow ? shift_of(m, k) - shift_of(a.m, k) : (a.m - m) * k.hi;
+  const float f = expf(d * kLn2);
+  a.t = f * fmaf(a.s, fmaxf(d, kFar), a.t);
+  a.s *= f;
   a.m = m;
 }
 
-template <bool kEnt, int N>
-__device__ __forceinline__ void soft_absorb(Soft& a, const float (&x)[N], const Base& k) {
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-  if (top > a.m) soft_raise<kEnt>(a, top, k);
+// x: unpacked columns, top: their maximum
+template <int N>
+__device__ __forceinline__ void soft_absorb(Soft& a, const float (&x)[N], float top, const Base& k) {
+  if (top > a.m) soft_raise(a, top, k);
   float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+  if (a.m > kLow) {
+    const float c = shift_of(a.m, k);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = k(x[i] - a.m), e = ex2(d);
-    s[i & 1] += e;
-    if (kEnt) t[i & 1] = fmaf(e, fmaxf(d, kFar), t[i & 1]);
+    for (int i = 0; i < N; ++i) {
+      const float d = at_least_far(fmaf(x[i], k.hi, c)), e = ex2(d);
+      s[i & 1] += e;
+      t[i & 1] = fmaf(e, d, t[i & 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = at_least_far((x[i] - a.m) * k.hi), e = ex2(d);
+      s[i & 1] += e;
+      t[i & 1] = fmaf(e, d, t[i & 1]);
+    }
   }
   a.s += s[0] + s[1];
-  if (kEnt) a.t += t[0] + t[1];
+  a.t += t[0] + t[1];
 }
 
-template <bool kEnt>
 __device__ __forceinline__ void soft_warp_reduce(Soft& a, const Base& k) {
   float m = a.m;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  soft_raise<kEnt>(a, m, k);
+  if (m > a.m) soft_raise(a, m, k);
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) {
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
-    if (kEnt) a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
   }
+}
+
+// What a row's sums say: ln sum_j e^((z_j - m) / T) = lns + fix, where lns is of the sums as they are and fix (about 1e-6)
+// what the rounding of c and of hi has shifted. Kept apart, and all in fp32: fp64 runs at a thirtieth of its rate.
+struct RowSoft {
+  float m, lns, fix;
+  float mean;  // of z - m under p
+  float entropy;
+};
+__device__ __forceinline__ RowSoft row_soft(const Soft& a, const Base& k) {
+  RowSoft r;
+  r.m = a.m;
+  const float off = a.m > kLow ? fmaf(a.m, k.hi, shift_of(a.m, k)) : 0.f;  // exact
+  r.lns = logf(a.s);
+  const float td = a.t / a.s;
+  r.mean = (td - off) / k.hi;
+  r.fix = kLn2 * fmaf(k.lo, r.mean, -off);
+  r.entropy = r.lns - td * kLn2;
+  return r;
+}
+__device__ __forceinline__ float row_logp(const RowSoft& r, float z, const Base& k) {
+  const float d = z - r.m;
+  return (isinf(d) ? d : fmaf(d, k.inv, d * k.inv_lack)) - r.lns - r.fix;
+}
+// What a gradient needs of a row: p_j = f 2^(z_j hi + c), f the rounding of c to a float; f < 0 marks a row of lowest
+// values: p_j = 2^((z_j - c) hi + 1 + f).
+__device__ __forceinline__ float2 row_shift(const RowSoft& r, const Base& k) {
+  constexpr float kE = 1.44269504f, kELack = 1.92596299e-8f;  // log2(e) as a sum
+  const float l = r.lns * kE, l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.fix * kE;
+  if (!(r.m > kLow)) return make_float2(r.m, -1.f - l);
+  const float p = r.m * k.hi, p_lack = fmaf(r.m, k.hi, -p);
+  const float c = -(p + l), t = -c - p;  // c's own rounding by the two-sum
+  const float lack = (p - (-c - t)) + (l - t) + p_lack + l_lack;
+  // what hi lacks at the mean of z; the columns around it differ by less than a rounding
+  return make_float2(c, exp2f(fmaf(k.lo, r.mean, -lack)));
 }
 
 // ---- the policy objective of one row ----------------------------------------------------------------------------------
 // Tie rules are torch's: the clamp passes its gradient on the closed interval, max() prefers the larger branch. NaN in
 // any input reaches the terms and the coefficient.
-__device__ __forceinline__ void policy_row(const PolicyTerms& q, int64_t row, float logp, float H, float w,
+struct PolicyIn {  // of one row; loaded before the row's sums, whose time hides the latency
+  float old_logp, adv, ref_logp;
+  __device__ __forceinline__ PolicyIn(const PolicyTerms& q, int64_t row)
+      : old_logp(q.old_logp[row]), adv(q.adv[row]), ref_logp(q.ref_logp ? q.ref_logp[row] : 0.f) {}
+};
+__device__ __forceinline__ void policy_row(const PolicyTerms& q, const PolicyIn& in, float logp, float H, float w,
                                            float4& terms, float2& coef) {
-  const float ratio = expf(logp - q.old_logp[row]);
-  const float na = -q.adv[row];
+  const float ratio = expf(logp - in.old_logp);
+  const float na = -in.adv;
   const float free = na * ratio;
   const float cut = na * fminf(fmaxf(ratio, q.clip_lo), q.clip_hi);
   const bool up = free > cut || isnan(free);
@@ -174,7 +247,7 @@ __device__ __forceinline__ void policy_row(const PolicyTerms& q, int64_t row, fl
   float a = open ? free : 0.f;
   float kl = 0.f;
   if (q.ref_logp != nullptr) {
-    const float d = q.ref_logp[row] - logp;
+    const float d = in.ref_logp - logp;
     float g;
     if (q.kl_kind == kKl1) {
       kl = -d, g = 1.f;
@@ -190,25 +263,159 @@ __device__ __forceinline__ void policy_row(const PolicyTerms& q, int64_t row, fl
   coef = make_float2(w * a, -q.entropy_coef * w);
 }
 
-// ---- row statistics ---------------------------------------------------------------------------------------------------
-constexpr int kStatThreads = 256;
-constexpr int kStatWarps = kStatThreads / 32;
+// ---- a row per CTA or cluster -------------------------------------------------------------------------------------------
+constexpr int kMostThreads = 512;
+constexpr int kMostWarps = kMostThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kFlight = 8;  // 16-byte loads that a thread has in flight
 
-// One cluster of CTAs per row (one CTA where there are enough rows), each CTA a share of the row's 16-byte vectors; the
-// shares' (m, s, t) meet in the first CTA's shared memory.
-template <typename T, bool kEnt>
-__global__ void __launch_bounds__(kStatThreads) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
-                                                                   bool policy, const Base k) {
+// A row's columns: up to VN - 1 single ones, 16-byte vectors, up to VN - 1 single ones.
+template <typename T>
+struct RowView {
+  const T* z;
+  const uint4* zv;
+  int head, nvec, tail;  // first column of the vectors, their number, first column behind them
+  __device__ __forceinline__ RowView(const T* row, int64_t vocab) : z(row) {
+    constexpr int VN = Elem<T>::kPerVec;
+    const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15u) / static_cast<int>(sizeof(T));
+    head = static_cast<int>(min(static_cast<int64_t>(mis ? VN - mis : 0), vocab));
+    nvec = static_cast<int>(vocab - head) / VN;
+    tail = head + nvec * VN;
+    zv = reinterpret_cast<const uint4*>(row + head);
+  }
+};
+
+// This thread's share of the row's sums. Eight loads are issued before the first is used: 128 KB in flight on a
+// multiprocessor of 1,024 threads.
+template <typename T>
+__device__ __forceinline__ Soft row_share(const RowView<T>& r, int64_t vocab, int rank, int ranks, const Base& k) {
+  constexpr int VN = Elem<T>::kPerVec;
+  constexpr int kChunk = 32 / VN;  // vectors of a step: 32 columns
+  const int threads = blockDim.x, step = ranks * threads;
+  const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
+  Soft acc{-FLT_MAX, 0.f, 0.f};
+  for (int i = rank * threads + threadIdx.x; i < r.nvec; i += kFlight * step) {
+    uint4 v[kFlight];
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) v[j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
+#pragma unroll
+    for (int j = 0; j < kFlight; j += kChunk) {
+      if (j > 0 && i + j * step >= r.nvec) continue;
+      float x[32], top = Elem<T>::top(v[j]);
+#pragma unroll
+      for (int n = 0; n < kChunk; ++n) {
+        Elem<T>::unpack(v[j + n], x + n * VN);
+        top = fmaxf(top, Elem<T>::top(v[j + n]));
+      }
+      soft_absorb(acc, x, top, k);
+    }
+  }
+  if (rank == 0 && threadIdx.x < 32 && (r.head > 0 || r.tail < vocab)) {
+    const int lane = threadIdx.x;
+    float x[2] = {-INFINITY, -INFINITY};
+    if (lane < r.head) x[0] = Elem<T>::get(r.z[lane]);
+    if (lane < static_cast<int>(vocab) - r.tail) x[1] = Elem<T>::get(r.z[r.tail + lane]);
+    soft_absorb(acc, x, fmaxf(x[0], x[1]), k);
+  }
+  return acc;
+}
+
+struct RowExchange {  // double-buffered: a row's buffers are free once the next row's barrier has been passed
+  Soft warp[2][kMostWarps];
+  Soft cta[2][kMaxCluster];
+};
+
+// Sums of the whole row, in warp 0 of every CTA of the cluster.
+__device__ __forceinline__ Soft row_total(Soft acc, RowExchange& x, int parity, int rank, int ranks, const Base& k,
+                                          const cg::cluster_group& cluster) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  soft_warp_reduce(acc, k);
+  if (warps > 1) {
+    if (lane == 0) x.warp[parity][warp] = acc;
+    __syncthreads();
+    if (warp == 0) {
+      acc = lane < warps ? x.warp[parity][lane] : Soft{-FLT_MAX, 0.f, 0.f};
+      soft_warp_reduce(acc, k);
+    }
+  }
+  if (ranks > 1) {
+    if (static_cast<int>(threadIdx.x) < ranks) *cluster.map_shared_rank(&x.cta[parity][rank], threadIdx.x) = acc;
+    cluster.sync();
+    if (warp == 0) {
+      acc = lane < ranks ? x.cta[parity][lane] : Soft{-FLT_MAX, 0.f, 0.f};
+      soft_warp_reduce(acc, k);
+    }
+  }
+  return acc;
+}
+
+// dz_j = a (delta_j - p_j) - b p_j (log p_j + H) of four or eight columns, a and b divided by T.
+struct RowGrad {
+  float2 cf;  // row_shift
+  float hi, a, c0, c1;
+  RowGrad() = default;
+  __device__ __forceinline__ RowGrad(const float2& shift, const Base& k, float a_, float b, float H)
+      : cf(shift), hi(k.hi), a(a_) {
+    const float f = cf.y > 0.f ? cf.y : 1.f;
+    c0 = -f * (a_ + b * (H + logf(f)));
+    c1 = -f * b * kLn2;
+  }
+  template <bool kEnt>
+  __device__ __forceinline__ float operator()(float z) const {
+    const float q = cf.y > 0.f ? fmaf(z, hi, cf.x) : (z - cf.x) * hi + 1.f + cf.y;
+    return ex2(q) * (kEnt ? fmaf(c1, fmaxf(q, kFar), c0) : c0);
+  }
+  template <typename T, bool kEnt>
+  __device__ __forceinline__ uint4 vec(const uint4& v, int col, int tok) const {
+    constexpr int VN = Elem<T>::kPerVec;
+    float x[VN];
+    Elem<T>::unpack(v, x);
+    if (cf.y > 0.f) {
+#pragma unroll
+      for (int e = 0; e < VN; ++e) {
+        const float q = fmaf(x[e], hi, cf.x);
+        x[e] = ex2(q) * (kEnt ? fmaf(c1, fmaxf(q, kFar), c0) : c0);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VN; ++e) x[e] = this->template operator()<kEnt>(x[e]);
+    }
+    if (static_cast<unsigned>(tok - col) < static_cast<unsigned>(VN)) {
+#pragma unroll
+      for (int e = 0; e < VN; ++e) x[e] += col + e == tok ? a : 0.f;
+    }
+    return Elem<T>::pack(x);
+  }
+  template <typename T, bool kEnt>
+  __device__ __forceinline__ T one(T z, int col, int tok) const {
+    const float g = this->template operator()<kEnt>(Elem<T>::get(z));
+    return Elem<T>::put(col == tok ? g + a : g);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ranks) {
+  const RowView<T> r(out, vocab);
+  uint4* ov = reinterpret_cast<uint4*>(out + r.head);
+  const int threads = blockDim.x;
+  for (int i = rank * threads + threadIdx.x; i < r.nvec; i += ranks * threads) __stcs(ov + i, make_uint4(0, 0, 0, 0));
+  if (rank == 0 && static_cast<int>(threadIdx.x) < r.head) out[threadIdx.x] = Elem<T>::put(0.f);
+  if (rank == 0 && static_cast<int>(threadIdx.x) < static_cast<int>(vocab) - r.tail) {
+    out[r.tail + threadIdx.x] = Elem<T>::put(0.f);
+  }
+}
+
+// ---- row statistics -----------------------------------------------------------------------------------------------------
+// A CTA per row, or a cluster of them where rows are few: each CTA a share of the row's vectors, whose sums meet in every
+// CTA's shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kMostThreads, 2) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
+                                                                      bool policy, const Base k) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
-  constexpr int VN = Elem<T>::kPerVec;
-  constexpr int kVecs = 16 / VN * 2;  // vectors in flight per thread: 32 elements
-  __shared__ Soft s_warp[kStatWarps];
-  __shared__ Soft s_cta[2][kMaxCluster];
+  __shared__ RowExchange x;
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int parity = 0;
   for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
     float w;
@@ -216,7 +423,7 @@ __global__ void __launch_bounds__(kStatThreads) token_stats_kernel(const TokenSt
     if (tok < 0) {
       if (rank == 0 && threadIdx.x == 0) {
         a.logp[row] = 0.f;
-        if (kEnt && a.entropy) a.entropy[row] = 0.f;
+        if (a.entropy) a.entropy[row] = 0.f;
         if (a.ml) a.ml[row] = make_float2(0.f, 0.f);
         if (policy) {
           a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -225,67 +432,116 @@ __global__ void __launch_bounds__(kStatThreads) token_stats_kernel(const TokenSt
       }
       continue;
     }
-    const T* z = row_ptr<const T>(a.z, row);
-    const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(z) & 15u) / static_cast<int>(sizeof(T));
-    const int64_t head = min(static_cast<int64_t>(mis ? VN - mis : 0), a.vocab);
-    const int64_t nvec = (a.vocab - head) / VN;
-    const int64_t tail = head + nvec * VN;
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-    Soft acc{-FLT_MAX, 0.f, 0.f};
-    if (rank == 0 && warp == 0) {  // at most VN - 1 elements before and behind the vectors
-      float x[2] = {-INFINITY, -INFINITY};
-      if (lane < head) x[0] = Elem<T>::get(z[lane]);
-      if (lane < a.vocab - tail) x[1] = Elem<T>::get(z[tail + lane]);
-      soft_absorb<kEnt>(acc, x, k);
-    }
-    const int64_t step = static_cast<int64_t>(ranks) * kStatThreads;
-    int64_t i = static_cast<int64_t>(rank) * kStatThreads + threadIdx.x;
-    for (; i + (kVecs - 1) * step < nvec; i += kVecs * step) {
-      uint4 v[kVecs];
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j) v[j] = __ldg(zv + i + j * step);
-      float x[kVecs * VN];
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j) Elem<T>::unpack(v[j], x + j * VN);
-      soft_absorb<kEnt>(acc, x, k);
-    }
-    for (; i < nvec; i += step) {
-      float x[VN];
-      Elem<T>::unpack(__ldg(zv + i), x);
-      soft_absorb<kEnt>(acc, x, k);
-    }
-    soft_warp_reduce<kEnt>(acc, k);
-    __syncthreads();  // the previous row's s_warp has been read
-    if (lane == 0) s_warp[warp] = acc;
-    __syncthreads();
-    if (warp == 0) {
-      acc = lane < kStatWarps ? s_warp[lane] : Soft{-FLT_MAX, 0.f, 0.f};
-      soft_warp_reduce<kEnt>(acc, k);
-    }
-    if (ranks > 1) {
-      if (threadIdx.x == 0) *cluster.map_shared_rank(&s_cta[parity][rank], 0) = acc;
-      cluster.sync();
-      if (rank == 0 && warp == 0) {
-        acc = lane < ranks ? s_cta[parity][lane] : Soft{-FLT_MAX, 0.f, 0.f};
-        soft_warp_reduce<kEnt>(acc, k);
-      }
-      parity ^= 1;
-    }
+    const RowView<T> r(row_ptr<const T>(a.z, row), a.vocab);
+    const float zt = Elem<T>::get(r.z[tok]);
+    const Soft acc = row_total(row_share(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
+    parity ^= 1;
     if (rank == 0 && threadIdx.x == 0) {
-      const float lns = logf(acc.s);
-      const float logp = static_cast<float>((Elem<T>::get(z[tok]) - acc.m) * a.inv_temp) - lns;
-      const float H = kEnt ? lns - acc.t / acc.s * kLn2 : 0.f;
+      const RowSoft soft = row_soft(acc, k);
+      const float logp = row_logp(soft, zt, k);
       a.logp[row] = logp;
-      if (kEnt && a.entropy) a.entropy[row] = H;
-      if (a.ml) a.ml[row] = make_float2(acc.m, log2f(acc.s));
+      if (a.entropy) a.entropy[row] = soft.entropy;
+      if (a.ml) a.ml[row] = row_shift(soft, k);
       if (policy) {
         float4 terms;
         float2 coef;
-        policy_row(q, row, logp, H, w, terms, coef);
+        policy_row(q, PolicyIn(q, row), logp, soft.entropy, w, terms, coef);
         a.terms[row] = terms;
         a.coef[row] = coef;
       }
     }
+  }
+}
+
+// ---- policy loss and gradient in one pass -------------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void block_sum(double (&x)[N], double* smem);
+
+// A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
+// the rows in work fit L2 (row_ranks), so the logits come from memory once.
+template <typename T, bool kEnt>
+__global__ void __launch_bounds__(kMostThreads, 2) token_policy_kernel(const TokenStatsArgs a, const PolicyTerms q,
+                                                                       const TokenRows grad, float scale,
+                                                                       const float* scale_device, int mean,
+                                                                       const Base k) {
+  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
+  griddep_launch_dependents();
+  constexpr int VN = Elem<T>::kPerVec;
+  __shared__ RowExchange x;
+  __shared__ double s_sum[kMostWarps];
+  __shared__ RowGrad s_grad[2];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int threads = blockDim.x;
+  if (scale_device) scale *= *scale_device;
+  if (mean) {  // every CTA sums the weights for itself, in the same order
+    double total[1] = {0.0};
+    for (int64_t r = threadIdx.x; r < a.rows; r += threads) {
+      float w;
+      row_token(a.idx, r, a.vocab, w);
+      total[0] += w;
+    }
+    block_sum(total, s_sum);
+    scale *= total[0] != 0.0 ? static_cast<float>(1.0 / total[0]) : 0.f;
+  }
+  const float factor = scale * k.inv;
+  int parity = 0;
+  for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
+    float w;
+    const int tok = static_cast<int>(row_token(a.idx, row, a.vocab, w));
+    T* out = row_ptr<T>(grad, row);
+    if (tok < 0) {
+      if (rank == 0 && threadIdx.x == 0) {
+        a.logp[row] = 0.f;
+        a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      zero_row(out, a.vocab, rank, ranks);
+      continue;
+    }
+    const RowView<T> r(row_ptr<const T>(a.z, row), a.vocab);
+    const PolicyIn in(q, row);
+    const float zt = Elem<T>::get(r.z[tok]);
+    const Soft acc = row_total(row_share(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
+    if (threadIdx.x < 32) {
+      const RowSoft soft = row_soft(acc, k);
+      const float logp = row_logp(soft, zt, k);
+      float4 terms;
+      float2 coef;
+      policy_row(q, in, logp, soft.entropy, w, terms, coef);
+      if (threadIdx.x == 0) {
+        s_grad[parity] = RowGrad(row_shift(soft, k), k, coef.x * factor, kEnt ? coef.y * factor : 0.f, soft.entropy);
+        if (rank == 0) {
+          a.logp[row] = logp;
+          a.terms[row] = terms;
+        }
+      }
+    }
+    __syncthreads();
+    const RowGrad g = s_grad[parity];
+    parity ^= 1;
+    if (g.a == 0.f && (!kEnt || g.c1 == 0.f)) {
+      zero_row(out, a.vocab, rank, ranks);
+      continue;
+    }
+    uint4* ov = reinterpret_cast<uint4*>(out + r.head);
+    const int step = ranks * threads;
+    for (int i = rank * threads + threadIdx.x; i < r.nvec; i += kFlight * step) {
+      uint4 v[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        if (i + j * step < r.nvec) v[j] = __ldg(r.zv + i + j * step);
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        const int n = i + j * step;
+        if (n < r.nvec) __stcs(ov + n, g.template vec<T, kEnt>(v[j], r.head + n * VN, tok));
+      }
+    }
+    if (rank == 0 && static_cast<int>(threadIdx.x) < r.head) {
+      out[threadIdx.x] = g.template one<T, kEnt>(r.z[threadIdx.x], threadIdx.x, tok);
+    }
+    const int end = r.tail + static_cast<int>(threadIdx.x);
+    if (rank == 0 && end < static_cast<int>(a.vocab)) out[end] = g.template one<T, kEnt>(r.z[end], end, tok);
   }
 }
 
@@ -300,56 +556,91 @@ Base base_of(double inv_temp) {
   const double k = inv_temp * kLog2e;
   Base b;
   b.hi = static_cast<float>(k);
-  if (static_cast<double>(b.hi) >= k) b.hi = std::nextafterf(b.hi, 0.f);
-  b.lo = static_cast<float>(k - static_cast<double>(b.hi));
-  b.inv_temp = static_cast<float>(inv_temp);
+  b.lo = static_cast<float>(k - b.hi);
+  b.inv = static_cast<float>(inv_temp);
+  b.inv_lack = static_cast<float>(inv_temp - b.inv);
   return b;
 }
 
-template <typename T, bool kEnt>
-cudaError_t launch_stats(const TokenStatsArgs& a, cudaStream_t stream) {
-  const int sms = sm_count();
-  // few rows: a row's vectors over up to 8 CTAs, while every thread keeps a vector and the CTAs stay within two an SM
-  int ranks = 1;
-  const int64_t nvec = a.vocab / Elem<T>::kPerVec;
-  while (ranks < kMaxCluster && a.rows * ranks * 2 <= 2 * sms && nvec >= 2 * ranks * kStatThreads) ranks *= 2;
-  const int64_t clusters = std::min<int64_t>(a.rows, static_cast<int64_t>(sms) * 64);
-  PolicyTerms q{};
-  if (a.policy) q = *a.policy;
+struct RowLaunch {
+  int threads, ranks;
+  int64_t clusters;
+};
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters * ranks));
-  cfg.blockDim = dim3(kStatThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(l.clusters * l.ranks));
+  cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(l.ranks);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, token_stats_kernel<T, kEnt>, a, q, a.policy != nullptr, base_of(a.inv_temp));
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Threads of a CTA: eight vectors each, 32 to 512. CTAs of a row: as many as leave every thread a vector while all rows
+// together stay within one wave; and with `again` (the row is read a second time) as many as keep the rows of a wave
+// within `kCached` bytes.
+constexpr int64_t kCached = 80 << 20;
+RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again, int waves) {
+  const int64_t sms = sm_count(), nvec = vocab * size / 16;
+  RowLaunch l;
+  l.threads = static_cast<int>(std::min<int64_t>(kMostThreads, std::max<int64_t>(32, (nvec / 8 + 31) / 32 * 32)));
+  const int64_t resident = std::min<int64_t>(1024 / l.threads, 32) * sms;
+  l.ranks = 1;
+  while (l.ranks < kMaxCluster && nvec >= 2 * l.ranks * l.threads) {
+    const bool idle = rows * l.ranks * 2 <= resident;
+    const bool large = again && std::min(rows, resident / l.ranks) * vocab * size > kCached;
+    if (!idle && !large) break;
+    l.ranks *= 2;
+  }
+  l.clusters = std::max<int64_t>(1, std::min(rows, waves * resident / l.ranks));
+  return l;
+}
+
+template <typename T>
+cudaError_t launch_stats(const TokenStatsArgs& a, cudaStream_t stream) {
+  PolicyTerms q{};
+  if (a.policy) q = *a.policy;
+  return launch_rows(token_stats_kernel<T>, row_launch(a.rows, a.vocab, sizeof(T), false, 32), stream, a, q,
+                     a.policy != nullptr, base_of(a.inv_temp));
+}
+
+template <typename T>
+cudaError_t launch_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
+                          cudaStream_t stream) {
+  const PolicyTerms q = *a.policy;
+  return launch_rows(q.entropy_coef != 0.f ? token_policy_kernel<T, true> : token_policy_kernel<T, false>,
+                     row_launch(a.rows, a.vocab, sizeof(T), true, 1), stream, a, q, grad, scale, scale_device, mean,
+                     base_of(a.inv_temp));
 }
 
 // ---- gradient of the logits from the row statistics -----------------------------------------------------------------------
 constexpr int kGradThreads = 256;
 constexpr int kGradVecs = 8;  // vectors per thread
 
-// dz_j = scale / T (a (delta_j - p_j) - b p_j (log p_j + H)); a block writes one row's segment of 16-byte vectors.
+// A block writes one row's segment of 16-byte vectors. Rows run backwards: the last ones that the statistics read are
+// still in L2.
 template <typename T, bool kEnt>
-__global__ void __launch_bounds__(kGradThreads) token_grad_kernel(const TokenGradArgs a, int64_t segs) {
+__global__ void __launch_bounds__(kGradThreads) token_grad_kernel(const TokenGradArgs a, int segs, const Base k) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
   constexpr int VN = Elem<T>::kPerVec;
-  const int64_t row = a.rows - 1 - blockIdx.x / segs, seg = blockIdx.x % segs;
+  const int64_t row = a.rows - 1 - blockIdx.x / segs;
+  const int seg = static_cast<int>(blockIdx.x % segs);
   T* out = row_ptr<T>(a.out, row);
   float w;
-  const int64_t tok = row_token(a.idx, row, a.vocab, w);
-  const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(out) & 15u) / static_cast<int>(sizeof(T));
-  const int64_t head = min(static_cast<int64_t>(mis ? VN - mis : 0), a.vocab);
-  const int64_t nvec = (a.vocab - head) / VN, tail = head + nvec * VN;
-  uint4* ov = reinterpret_cast<uint4*>(out + head);
-  const int64_t v0 = seg * (kGradThreads * kGradVecs), v1 = min(nvec, v0 + kGradThreads * kGradVecs);
+  const int tok = static_cast<int>(row_token(a.idx, row, a.vocab, w));
+  const RowView<T> o(out, a.vocab);
+  uint4* ov = reinterpret_cast<uint4*>(out + o.head);
+  const int v0 = seg * (kGradThreads * kGradVecs) + threadIdx.x, v1 = min(o.nvec, (seg + 1) * (kGradThreads * kGradVecs));
+  const int end = o.tail + static_cast<int>(threadIdx.x);
   float ca = 0.f, cb = 0.f;
   if (tok >= 0) {
     float f = static_cast<float>(a.scale * a.inv_temp);
@@ -360,57 +651,37 @@ __global__ void __launch_bounds__(kGradThreads) token_grad_kernel(const TokenGra
     if (kEnt) cb = a.b[row * a.b_stride] * f;
   }
   if (tok < 0 || (ca == 0.f && (!kEnt || cb == 0.f))) {  // nothing to read
-    for (int64_t i = v0 + threadIdx.x; i < v1; i += kGradThreads) ov[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (seg == 0 && threadIdx.x < head) out[threadIdx.x] = Elem<T>::put(0.f);
-    if (seg == 0 && threadIdx.x < a.vocab - tail) out[tail + threadIdx.x] = Elem<T>::put(0.f);
+    for (int i = v0; i < v1; i += kGradThreads) __stcs(ov + i, make_uint4(0u, 0u, 0u, 0u));
+    if (seg == 0 && static_cast<int>(threadIdx.x) < o.head) out[threadIdx.x] = Elem<T>::put(0.f);
+    if (seg == 0 && end < static_cast<int>(a.vocab)) out[end] = Elem<T>::put(0.f);
     return;
   }
   const T* z = row_ptr<const T>(a.z, row);
-  const float2 ml = a.ml[row];
-  const float k = static_cast<float>(a.inv_temp * kLog2e);
-  const float H = kEnt ? a.entropy[row] : 0.f;
-  const float c0 = -ca - cb * H, c1 = -cb * kLn2;
-  auto grad = [&](float x, int64_t col) {
-    const float lp = (x - ml.x) * k - ml.y;  // log2 p
-    const float p = ex2(lp);
-    float g = p * (kEnt ? fmaf(c1, fmaxf(lp, kFar), c0) : c0);
-    return col == tok ? g + ca : g;
-  };
-  if (seg == 0 && threadIdx.x < head) out[threadIdx.x] = Elem<T>::put(grad(Elem<T>::get(z[threadIdx.x]), threadIdx.x));
-  if (seg == 0 && threadIdx.x < a.vocab - tail) {
-    const int64_t col = tail + threadIdx.x;
-    out[col] = Elem<T>::put(grad(Elem<T>::get(z[col]), col));
+  const RowGrad g(a.ml[row], k, ca, cb, kEnt ? a.entropy[row] : 0.f);
+  if (seg == 0 && static_cast<int>(threadIdx.x) < o.head) {
+    out[threadIdx.x] = g.template one<T, kEnt>(z[threadIdx.x], threadIdx.x, tok);
   }
+  if (seg == 0 && end < static_cast<int>(a.vocab)) out[end] = g.template one<T, kEnt>(z[end], end, tok);
   const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   if (same) {
-    const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+    const uint4* zv = reinterpret_cast<const uint4*>(z + o.head);
+    uint4 v[kGradVecs];
 #pragma unroll
-    for (int h = 0; h < kGradVecs; h += 4) {
-      uint4 v[4];
+    for (int j = 0; j < kGradVecs; ++j) {
+      if (v0 + j * kGradThreads < v1) v[j] = __ldg(zv + v0 + j * kGradThreads);
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t i = v0 + (h + j) * kGradThreads + threadIdx.x;
-        if (i < v1) v[j] = __ldg(zv + i);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t i = v0 + (h + j) * kGradThreads + threadIdx.x;
-        if (i >= v1) continue;
-        float x[VN];
-        Elem<T>::unpack(v[j], x);
-        const int64_t col = head + i * VN;
-#pragma unroll
-        for (int e = 0; e < VN; ++e) x[e] = grad(x[e], col + e);
-        ov[i] = Elem<T>::pack(x);
-      }
+    for (int j = 0; j < kGradVecs; ++j) {
+      const int i = v0 + j * kGradThreads;
+      if (i < v1) __stcs(ov + i, g.template vec<T, kEnt>(v[j], o.head + i * VN, tok));
     }
   } else {  // rows of input and output start at different places within 16 bytes
-    for (int64_t i = v0 + threadIdx.x; i < v1; i += kGradThreads) {
-      const int64_t col = head + i * VN;
+    for (int i = v0; i < v1; i += kGradThreads) {
+      const int col = o.head + i * VN;
       float x[VN];
 #pragma unroll
-      for (int e = 0; e < VN; ++e) x[e] = grad(Elem<T>::get(z[col + e]), col + e);
-      ov[i] = Elem<T>::pack(x);
+      for (int e = 0; e < VN; ++e) x[e] = Elem<T>::get(z[col + e]);
+      __stcs(ov + i, g.template vec<T, kEnt>(Elem<T>::pack(x), col, tok));
     }
   }
 }
@@ -420,8 +691,8 @@ cudaError_t launch_grad(const TokenGradArgs& a, cudaStream_t stream) {
   constexpr int64_t per = static_cast<int64_t>(kGradThreads) * kGradVecs * Elem<T>::kPerVec;
   const int64_t segs = std::max<int64_t>(1, (a.vocab + per - 1) / per);
   const dim3 grid(static_cast<unsigned>(a.rows * segs));
-  if (a.b) return launch_pdl(token_grad_kernel<T, true>, grid, dim3(kGradThreads), 0, stream, a, segs);
-  return launch_pdl(token_grad_kernel<T, false>, grid, dim3(kGradThreads), 0, stream, a, segs);
+  return launch_pdl(a.b ? token_grad_kernel<T, true> : token_grad_kernel<T, false>, grid, dim3(kGradThreads), 0, stream, a,
+                    static_cast<int>(segs), base_of(a.inv_temp));
 }
 
 // ---- sums over rows, sequences and pairs -----------------------------------------------------------------------------------
@@ -547,12 +818,20 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
 
 cudaError_t token_stats(const TokenStatsArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
-  const bool ent = a.entropy != nullptr;
   switch (a.dtype) {
-    case kTokF32: return ent ? launch_stats<float, true>(a, stream) : launch_stats<float, false>(a, stream);
-    case kTokBF16:
-      return ent ? launch_stats<__nv_bfloat16, true>(a, stream) : launch_stats<__nv_bfloat16, false>(a, stream);
-    default: return ent ? launch_stats<__half, true>(a, stream) : launch_stats<__half, false>(a, stream);
+    case kTokF32: return launch_stats<float>(a, stream);
+    case kTokBF16: return launch_stats<__nv_bfloat16>(a, stream);
+    default: return launch_stats<__half>(a, stream);
+  }
+}
+
+cudaError_t token_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
+                         cudaStream_t stream) {
+  if (a.rows == 0) return cudaSuccess;
+  switch (a.dtype) {
+    case kTokF32: return launch_policy<float>(a, grad, scale, scale_device, mean, stream);
+    case kTokBF16: return launch_policy<__nv_bfloat16>(a, grad, scale, scale_device, mean, stream);
+    default: return launch_policy<__half>(a, grad, scale, scale_device, mean, stream);
   }
 }
 

@@ -44,12 +44,17 @@ struct TokenStatsArgs {
   double inv_temp;
   float* logp;      // [rows]
   float* entropy;   // [rows]; null: not computed
-  float2* ml;       // [rows] (m, log2 s); null: not stored
+  float2* ml;       // [rows] what token_grad needs; null: not stored
   const PolicyTerms* policy;  // null: log-probabilities only (host pointer, copied into the launch)
   float4* terms;    // [rows] weighted (surrogate, kl, entropy, clipped) with `policy`
   float2* coef;     // [rows] (dL/dlogp, dL/dH) times the row's weight, before division by the sum of weights
 };
 cudaError_t token_stats(const TokenStatsArgs& a, cudaStream_t stream);
+// The statistics with `policy` and the gradient times scale (times *scale_device) in one pass; with `mean` the gradient is
+// divided by the sum of the weights. `grad` rows start at the same places within 16 bytes as the logits' rows. Writes logp
+// and terms.
+cudaError_t token_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
+                         cudaStream_t stream);
 
 struct TokenGradArgs {
   int dtype;
