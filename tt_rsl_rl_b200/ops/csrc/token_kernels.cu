@@ -7,6 +7,8 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <mutex>
+#include <vector>
 
 #include "sm100_primitives.cuh"
 #include "token_kernels.cuh"
@@ -104,7 +106,9 @@ struct Elem<__half> {
 
 template <typename T>
 __device__ __forceinline__ T* row_ptr(const TokenRows& r, int64_t row) {
-  const int64_t o = row / r.inner, i = row - o * r.inner;
+  if (row < r.inner) return static_cast<T*>(r.base) + row * r.stride_inner;
+  const uint32_t o = static_cast<uint32_t>(row) / static_cast<uint32_t>(r.inner);  // rows are below 2^31
+  const uint32_t i = static_cast<uint32_t>(row) - o * static_cast<uint32_t>(r.inner);
   return static_cast<T*>(r.base) + o * r.stride_outer + i * r.stride_inner;
 }
 
@@ -233,6 +237,8 @@ __device__ __forceinline__ float2 row_shift(const RowSoft& r, const Base& k) {
 // any input reaches the terms and the coefficient.
 struct PolicyIn {  // of one row; loaded before the row's sums, whose time hides the latency
   float old_logp, adv, ref_logp;
+  __device__ __forceinline__ PolicyIn(float old, float advantage, float ref)
+      : old_logp(old), adv(advantage), ref_logp(ref) {}
   __device__ __forceinline__ PolicyIn(const PolicyTerms& q, int64_t row)
       : old_logp(q.old_logp[row]), adv(q.adv[row]), ref_logp(q.ref_logp ? q.ref_logp[row] : 0.f) {}
 };
@@ -545,6 +551,359 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_policy_kernel(const Tok
   }
 }
 
+// ---- the same with the row in shared memory ------------------------------------------------------------------------------
+// A cluster of CTAs holds a row, each CTA a slice of it. Eight warps turn slices into their gradients in place; one warp
+// moves slices, by bulk copies into a ring of stages and out of them; one warp does what a row needs once: it joins the
+// sums, exchanges them with the other CTAs and works out the coefficients. The eight warps sum row n + 1 before they turn
+// to the gradient of row n, which gives the exchange the time of a row. The logits are read once and the gradient written
+// once, both without registers.
+constexpr int kRingWarps = 8;
+constexpr int kRingThreads = kRingWarps * 32;  // that compute
+constexpr int kStages = 3;
+
+struct RingItem {  // one row of a stage
+  int64_t row;     // -1: no more rows
+  int tok;         // -1: the row does not count
+  float w, zt, old_logp, adv, ref_logp;
+};
+struct RingShared {
+  uint64_t full[kStages], done[kStages];  // a stage's slice has arrived / has been used
+  uint64_t summed[2], met[2], ready[2];   // a row's sums: of the warps, of the CTAs; its coefficients
+  RingItem item[kStages];
+  Soft warp[2][kRingWarps];
+  float4 cta[2][kMaxCluster];
+  RowGrad grad[2];
+  int lost;  // a wait ran out of time: nothing waits any more, the losses become NaN
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
+  uint32_t y;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(smem_u32(p)), "r"(rank));
+  return y;
+}
+// Puts v into a peer's slot and arrives at the peer's barrier.
+__device__ __forceinline__ void peer_put(uint32_t slot, uint32_t bar, const Soft& v) {
+  asm volatile(
+      "st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %3};\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%4];\n" ::"r"(slot),
+      "f"(v.m), "f"(v.s), "f"(v.t), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool peer_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits for a phase, at most kWaitTimeoutNs, and not at all once a wait has failed.
+__device__ __forceinline__ void ring_wait(RingShared& sh, uint64_t* bar, uint32_t parity) {
+  if (peer_try_wait(bar, parity)) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (!peer_try_wait(bar, parity)) {
+    if (*const_cast<volatile int*>(&sh.lost) || globaltimer_ns() - t0 > kWaitTimeoutNs) {
+      *const_cast<volatile int*>(&sh.lost) = 1;
+      return;
+    }
+  }
+}
+// The same answer in every lane.
+__device__ __forceinline__ bool ring_lost(const RingShared& sh) {
+  return __any_sync(__activemask(), *const_cast<volatile const int*>(&sh.lost) != 0);
+}
+
+template <typename T>
+struct Slice {  // this CTA's vectors of a row
+  int v0, v1;
+  __device__ __forceinline__ Slice(const RowView<T>& r, int rank, int ranks) {
+    const int shift = 31 - __clz(ranks);                         // ranks are a power of two
+    const int per = (((r.nvec + ranks - 1) >> shift) + 7) & ~7;  // whole 128-byte lines
+    v0 = min(rank * per, r.nvec);
+    v1 = min(v0 + per, r.nvec);
+  }
+};
+
+struct RingCursor {  // walks the stages of the ring
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) stage = 0, parity ^= 1u;
+  }
+};
+
+// The mover: one thread. It looks rows up stages ahead of the arithmetic, starts their copies, and sends gradients off.
+template <typename T>
+__device__ __forceinline__ void ring_move(const TokenStatsArgs& a, const PolicyTerms& q, const TokenRows& grad,
+                                          RingShared& sh, uint8_t* ring, int stage_bytes, int rank, int ranks) {
+  const int64_t row_step = gridDim.x / ranks;
+  int64_t row = blockIdx.x / ranks;
+  auto look = [&](int64_t r) {
+    RingItem it;
+    it.row = r < a.rows ? r : -1;
+    it.tok = -1;
+    if (it.row < 0) return it;
+    it.tok = static_cast<int>(row_token(a.idx, r, a.vocab, it.w));
+    if (it.tok < 0) return it;
+    const PolicyIn in(q, r);
+    it.old_logp = in.old_logp, it.adv = in.adv, it.ref_logp = in.ref_logp;
+    it.zt = Elem<T>::get(row_ptr<const T>(a.z, r)[it.tok]);
+    return it;
+  };
+  auto publish = [&](int s, const RingItem& it) {
+    sh.item[s] = it;
+    if (it.tok < 0) {
+      mbar_arrive(&sh.full[s]);
+      return;
+    }
+    const RowView<T> r(row_ptr<const T>(a.z, it.row), a.vocab);
+    const Slice<T> sl(r, rank, ranks);
+    const uint32_t bytes = static_cast<uint32_t>(sl.v1 - sl.v0) * 16u;
+    mbar_arrive_expect_tx(&sh.full[s], bytes);
+    if (bytes) bulk_load(ring + s * stage_bytes, r.zv + sl.v0, bytes, &sh.full[s]);
+  };
+  for (int s = 0; s < kStages; ++s, row += row_step) publish(s, look(row));
+  for (RingCursor c;; c.next(), row += row_step) {
+    const RingItem next = look(row);
+    const RingItem it = sh.item[c.stage];
+    if (it.row < 0) break;
+    ring_wait(sh, &sh.done[c.stage], c.parity);
+    if (ring_lost(sh)) {  // no more copies; those under way end before the memory does
+      for (int s = 0; s < kStages; ++s, c.next()) mbar_wait(&sh.full[c.stage], c.parity);
+      break;
+    }
+    if (it.tok >= 0) {
+      T* out = row_ptr<T>(grad, it.row);
+      const RowView<T> r(out, a.vocab);
+      const Slice<T> sl(r, rank, ranks);
+      if (sl.v1 > sl.v0) {
+        bulk_store(out + r.head + static_cast<int64_t>(sl.v0) * Elem<T>::kPerVec, ring + c.stage * stage_bytes,
+                   static_cast<uint32_t>(sl.v1 - sl.v0) * 16u);
+      }
+      bulk_commit_group();
+      bulk_wait_group_read<0>();
+    }
+    publish(c.stage, next);
+  }
+}
+
+// What a row needs once: one warp.
+template <typename T, bool kEnt>
+__device__ __forceinline__ void ring_join(const TokenStatsArgs& a, const PolicyTerms& q, float scale,
+                                          const float* scale_device, int mean, const Base& k, RingShared& sh, int rank,
+                                          int ranks) {
+  const int lane = threadIdx.x & 31;
+  if (scale_device) scale *= *scale_device;
+  if (mean) {  // every CTA sums the weights for itself, in the same order
+    double total = 0.0;
+    for (int64_t r = lane; r < a.rows; r += 32) {
+      float w;
+      row_token(a.idx, r, a.vocab, w);
+      total += w;
+    }
+    for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    scale *= total != 0.0 ? static_cast<float>(1.0 / total) : 0.f;
+  }
+  const float factor = scale * k.inv;
+  uint32_t rounds = 0;
+  for (RingCursor c;; c.next()) {
+    ring_wait(sh, &sh.full[c.stage], c.parity);
+    if (ring_lost(sh)) break;
+    const RingItem it = sh.item[c.stage];
+    if (it.row < 0) break;
+    if (it.tok < 0) {
+      if (rank == 0 && lane == 0) {
+        a.logp[it.row] = 0.f;
+        a.terms[it.row] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.done[c.stage]);
+      continue;
+    }
+    const int b = rounds & 1;
+    const uint32_t phase = (rounds >> 1) & 1;
+    ++rounds;
+    ring_wait(sh, &sh.summed[b], phase);
+    Soft acc = lane < kRingWarps ? sh.warp[b][lane] : Soft{-FLT_MAX, 0.f, 0.f};
+    soft_warp_reduce(acc, k);
+    if (ranks > 1) {
+      // a slot is free: a peer that sends its sums of this row has read those of the row before last
+      if (lane < ranks) peer_put(peer_address(&sh.cta[b][rank], lane), peer_address(&sh.met[b], lane), acc);
+      ring_wait(sh, &sh.met[b], phase);
+      const float4 p = sh.cta[b][lane < ranks ? lane : 0];
+      acc = lane < ranks ? Soft{p.x, p.y, p.z} : Soft{-FLT_MAX, 0.f, 0.f};
+      soft_warp_reduce(acc, k);
+    }
+    const RowSoft soft = row_soft(acc, k);
+    const float logp = row_logp(soft, it.zt, k);
+    float4 terms;
+    float2 coef;
+    policy_row(q, PolicyIn(it.old_logp, it.adv, it.ref_logp), logp, soft.entropy, it.w, terms, coef);
+    const RowGrad g(row_shift(soft, k), k, coef.x * factor, kEnt ? coef.y * factor : 0.f, soft.entropy);
+    if (ring_lost(sh)) terms.x = __int_as_float(0x7fffffff);
+    if (lane == 0) {
+      sh.grad[b] = g;
+      mbar_arrive(&sh.ready[b]);
+      mbar_arrive(&sh.done[c.stage]);
+      if (rank == 0) {
+        a.logp[it.row] = logp;
+        a.terms[it.row] = terms;
+      }
+    }
+  }
+}
+
+// The arithmetic: eight warps.
+template <typename T, bool kEnt>
+__device__ __forceinline__ void ring_compute(const TokenStatsArgs& a, const TokenRows& grad, const Base& k,
+                                             RingShared& sh, uint8_t* ring, int stage_bytes, int rank, int ranks) {
+  constexpr int VN = Elem<T>::kPerVec;
+  constexpr int kChunk = 32 / VN;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
+
+  auto sum = [&](int stage, const RingItem& it, int b) {
+    const RowView<T> r(row_ptr<const T>(a.z, it.row), a.vocab);
+    const Slice<T> sl(r, rank, ranks);
+    const int count = sl.v1 - sl.v0;
+    const uint4* v = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
+    Soft acc{-FLT_MAX, 0.f, 0.f};
+    for (int i = threadIdx.x; i < count; i += kChunk * kRingThreads) {
+      uint4 c[kChunk];
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) c[j] = i + j * kRingThreads < count ? v[i + j * kRingThreads] : none;
+      float x[32], top = Elem<T>::top(c[0]);
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        Elem<T>::unpack(c[j], x + j * VN);
+        top = fmaxf(top, Elem<T>::top(c[j]));
+      }
+      soft_absorb(acc, x, top, k);
+    }
+    if (rank == 0 && warp == 0 && (r.head > 0 || r.tail < a.vocab)) {  // columns before and behind the vectors
+      float x[2] = {-INFINITY, -INFINITY};
+      if (lane < r.head) x[0] = Elem<T>::get(r.z[lane]);
+      if (lane < static_cast<int>(a.vocab) - r.tail) x[1] = Elem<T>::get(r.z[r.tail + lane]);
+      soft_absorb(acc, x, fmaxf(x[0], x[1]), k);
+    }
+    soft_warp_reduce(acc, k);
+    if (lane == 0) {
+      sh.warp[b][warp] = acc;
+      mbar_arrive(&sh.summed[b]);
+    }
+  };
+
+  auto turn = [&](int stage, const RingItem& it, int b) {
+    T* out = row_ptr<T>(grad, it.row);
+    const RowView<T> r(out, a.vocab);  // starts where the logits' row does within 16 bytes
+    const Slice<T> sl(r, rank, ranks);
+    const int count = sl.v1 - sl.v0;
+    const int end = r.tail + static_cast<int>(threadIdx.x);
+    const bool before = rank == 0 && static_cast<int>(threadIdx.x) < r.head;
+    const bool behind = rank == 0 && end < static_cast<int>(a.vocab);
+    if (it.tok < 0) {
+      uint4* ov = reinterpret_cast<uint4*>(out + r.head) + sl.v0;
+      for (int i = threadIdx.x; i < count; i += kRingThreads) __stcs(ov + i, make_uint4(0, 0, 0, 0));
+      if (before) out[threadIdx.x] = Elem<T>::put(0.f);
+      if (behind) out[end] = Elem<T>::put(0.f);
+      return;
+    }
+    const RowGrad g = sh.grad[b];
+    uint4* v = reinterpret_cast<uint4*>(ring + stage * stage_bytes);
+    const int col = r.head + sl.v0 * VN;
+    for (int i = threadIdx.x; i < count; i += 4 * kRingThreads) {
+      uint4 c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j * kRingThreads < count) c[j] = v[i + j * kRingThreads];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = i + j * kRingThreads;
+        if (at < count) v[at] = g.template vec<T, kEnt>(c[j], col + at * VN, it.tok);
+      }
+    }
+    const T* z = row_ptr<const T>(a.z, it.row);
+    if (before) out[threadIdx.x] = g.template one<T, kEnt>(z[threadIdx.x], threadIdx.x, it.tok);
+    if (behind) out[end] = g.template one<T, kEnt>(z[end], end, it.tok);
+    fence_proxy_async_smem();
+  };
+
+  RingCursor ahead, here;
+  uint32_t sums = 0, turns = 0;
+  RingItem now, next;
+  auto fetch = [&](RingItem& it) {  // the item ahead, and its sums
+    ring_wait(sh, &sh.full[ahead.stage], ahead.parity);
+    it = sh.item[ahead.stage];
+    if (ring_lost(sh)) it.row = -1;
+    if (it.row >= 0 && it.tok >= 0) sum(ahead.stage, it, sums++ & 1);
+    if (it.row >= 0) ahead.next();
+  };
+  fetch(now);
+  while (now.row >= 0) {
+    fetch(next);
+    const int b = turns & 1;
+    if (now.tok >= 0) {
+      ring_wait(sh, &sh.ready[b], (turns >> 1) & 1);
+      ++turns;
+    }
+    if (ring_lost(sh)) break;
+    turn(here.stage, now, b);
+    mbar_arrive(&sh.done[here.stage]);
+    here.next();
+    now = next;
+  }
+}
+
+template <typename T, bool kEnt>
+__global__ void __launch_bounds__(kRingThreads + 64, 2) token_policy_ring_kernel(
+    const TokenStatsArgs a, const PolicyTerms q, const TokenRows grad, float scale, const float* scale_device, int mean,
+    const Base k, int stage_bytes) {
+  griddep_wait();  // launched with programmatic stream serialization
+  griddep_launch_dependents();
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ RingShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.done[s], kRingThreads + 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh.summed[b], kRingWarps);
+      mbar_init(&sh.met[b], ranks);
+      mbar_init(&sh.ready[b], 1);
+    }
+    sh.lost = 0;
+    fence_mbar_init();
+  }
+  cluster.sync();  // the barriers of every CTA are ready
+  const int warp = threadIdx.x >> 5;
+  if (warp < kRingWarps) {
+    ring_compute<T, kEnt>(a, grad, k, sh, ring, stage_bytes, rank, ranks);
+  } else if (warp == kRingWarps) {
+    ring_join<T, kEnt>(a, q, scale, scale_device, mean, k, sh, rank, ranks);
+  } else {
+    if ((threadIdx.x & 31) == 0) ring_move<T>(a, q, grad, sh, ring, stage_bytes, rank, ranks);
+    __syncwarp();
+  }
+  cluster.sync();  // no CTA leaves while another may still write into it
+}
+
 int sm_count() {
   int dev = 0, n = 148;
   cudaGetDevice(&dev);
@@ -562,18 +921,22 @@ Base base_of(double inv_temp) {
   return b;
 }
 
+// Rows from 8 KB up to 8 slices of 72 KB go through shared memory: slices of at most 32 KB where eight CTAs can hold the row
+// that way (two CTAs a multiprocessor), else of at most 72 KB (one).
+constexpr int64_t kRingLeast = 8 << 10, kRingSlice = 32 << 10, kRingMost = 72 << 10;
+
 struct RowLaunch {
   int threads, ranks;
   int64_t clusters;
+  int smem = 0;
 };
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t stream, Args&&... args) {
+cudaLaunchConfig_t row_config(const RowLaunch& l, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.clusters * l.ranks));
   cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(l.smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(l.ranks);
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -581,6 +944,47 @@ cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cfg;
+}
+
+// Clusters of a kernel that fit the device at once (a cluster stays within a group of multiprocessors, so fewer than
+// their number suggests; one cluster too many would be a second wave). Asked once per shape and device.
+template <typename Kern>
+cudaError_t resident_clusters(Kern kern, const RowLaunch& l, int* count) {
+  struct Known {
+    const void* kern;
+    int device, ranks, smem, count;
+  };
+  static std::mutex lock;
+  static std::vector<Known> known;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const std::lock_guard<std::mutex> guard(lock);
+  for (const Known& x : known) {
+    if (x.kern == reinterpret_cast<const void*>(kern) && x.device == device && x.ranks == l.ranks && x.smem == l.smem) {
+      *count = x.count;
+      return cudaSuccess;
+    }
+  }
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingMost) * kStages);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  RowLaunch one = l;
+  one.clusters = 1;
+  cudaLaunchConfig_t cfg = row_config(one, nullptr, attr);
+  cfg.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(count, kern, &cfg);
+  if (e != cudaSuccess) return e;
+  *count = std::max(*count, 1);
+  known.push_back({reinterpret_cast<const void*>(kern), device, l.ranks, l.smem, *count});
+  return cudaSuccess;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = row_config(l, stream, attr);
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
@@ -616,9 +1020,29 @@ template <typename T>
 cudaError_t launch_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
                           cudaStream_t stream) {
   const PolicyTerms q = *a.policy;
-  return launch_rows(q.entropy_coef != 0.f ? token_policy_kernel<T, true> : token_policy_kernel<T, false>,
-                     row_launch(a.rows, a.vocab, sizeof(T), true, 1), stream, a, q, grad, scale, scale_device, mean,
-                     base_of(a.inv_temp));
+  const bool ent = q.entropy_coef != 0.f;
+  const int64_t bytes = a.vocab * static_cast<int64_t>(sizeof(T)), sms = sm_count();
+  const auto slice = [&](int64_t ranks) { return ((bytes / 16 + ranks - 1) / ranks + 7) / 8 * 128; };
+  if (bytes < kRingLeast || slice(kMaxCluster) > kRingMost) {
+    return launch_rows(ent ? token_policy_kernel<T, true> : token_policy_kernel<T, false>,
+                       row_launch(a.rows, a.vocab, sizeof(T), true, 1), stream, a, q, grad, scale, scale_device, mean,
+                       base_of(a.inv_temp));
+  }
+  RowLaunch l;
+  l.threads = kRingThreads + 64;
+  l.ranks = 1;
+  while (l.ranks < kMaxCluster &&
+         (slice(l.ranks) > kRingSlice || (a.rows * l.ranks * 2 <= 2 * sms && slice(l.ranks) >= 16 * kRingThreads * 2))) {
+    l.ranks *= 2;
+  }
+  const int stage = static_cast<int>(slice(l.ranks));
+  l.smem = stage * kStages;
+  const auto kern = ent ? token_policy_ring_kernel<T, true> : token_policy_ring_kernel<T, false>;
+  int resident = 0;
+  const cudaError_t e = resident_clusters(kern, l, &resident);
+  if (e != cudaSuccess) return e;
+  l.clusters = std::min<int64_t>(a.rows, resident);
+  return launch_rows(kern, l, stream, a, q, grad, scale, scale_device, mean, base_of(a.inv_temp), stage);
 }
 
 // ---- gradient of the logits from the row statistics -----------------------------------------------------------------------
@@ -691,8 +1115,10 @@ cudaError_t launch_grad(const TokenGradArgs& a, cudaStream_t stream) {
   constexpr int64_t per = static_cast<int64_t>(kGradThreads) * kGradVecs * Elem<T>::kPerVec;
   const int64_t segs = std::max<int64_t>(1, (a.vocab + per - 1) / per);
   const dim3 grid(static_cast<unsigned>(a.rows * segs));
-  return launch_pdl(a.b ? token_grad_kernel<T, true> : token_grad_kernel<T, false>, grid, dim3(kGradThreads), 0, stream, a,
-                    static_cast<int>(segs), base_of(a.inv_temp));
+  const Base k = base_of(a.inv_temp);
+  const int n = static_cast<int>(segs);
+  if (a.b) return launch_pdl(token_grad_kernel<T, true>, grid, dim3(kGradThreads), 0, stream, a, n, k);
+  return launch_pdl(token_grad_kernel<T, false>, grid, dim3(kGradThreads), 0, stream, a, n, k);
 }
 
 // ---- sums over rows, sequences and pairs -----------------------------------------------------------------------------------
