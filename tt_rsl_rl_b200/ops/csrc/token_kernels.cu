@@ -34,6 +34,43 @@ __device__ __forceinline__ float at_least_far(float d) {  // a NaN stays one
   return y;
 }
 
+// Two fp32 numbers in one instruction (sm_100): what these kernels issue, not what they compute, is their limit.
+struct Pair {
+  unsigned long long v;
+  Pair() = default;
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void split(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return y;
+}
+__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
+  Pair y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+  return y;
+}
+__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
+  Pair y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+  return y;
+}
+__device__ __forceinline__ Pair ex2(const Pair& x) {
+  float lo, hi;
+  x.split(lo, hi);
+  return Pair(ex2(lo), ex2(hi));
+}
+
+// Below this maximum c overflows: rows of lowest values subtract first. In the other rows a column below it counts as it:
+// its probability is zero, and that zero's products stay numbers.
+constexpr float kLow = -73786976294838206464.f;  // -2^66
+__device__ __forceinline__ float at_least_low(float z) {  // a NaN stays one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(z), "f"(kLow));
+  return y;
+}
+
 template <typename T>
 struct Elem;
 template <>
@@ -42,6 +79,11 @@ struct Elem<float> {
   static constexpr uint32_t kNone = 0xff800000u;  // -inf
   static __device__ __forceinline__ float top(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ void unpack_low(const uint4& v, float* x) {
+    unpack(v, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = at_least_low(x[i]);
   }
   static __device__ __forceinline__ float get(float x) { return x; }
   static __device__ __forceinline__ float put(float x) { return x; }
@@ -60,6 +102,13 @@ struct Elem<__nv_bfloat16> {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ void unpack_low(uint4 v, float* x) {
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+    const __nv_bfloat162 low = __float2bfloat162_rn(kLow);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+    unpack(v, x);
   }
   static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
@@ -84,6 +133,11 @@ struct Elem<__half> {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
     const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ void unpack_low(const uint4& v, float* x) {
+    unpack(v, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = at_least_low(x[i]);
   }
   static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
@@ -147,8 +201,6 @@ struct Base {
   float inv, inv_lack;  // 1 / T as a sum
 };
 
-constexpr float kLow = -1e30f;  // below this maximum c overflows; such rows (only lowest values) subtract first
-
 __device__ __forceinline__ float shift_of(float m, const Base& k) { return -m * k.hi; }
 
 // Rare, so by the accurate function: a chain of these with ex2.approx, which is low by 5e-8 on average, shows in sums.
@@ -160,29 +212,58 @@ __device__ __forceinline__ void soft_raise(Soft& a, float m, const Base& k) {
   a.m = m;
 }
 
-// x: unpacked columns, top: their maximum
-template <int N>
-__device__ __forceinline__ void soft_absorb(Soft& a, const float (&x)[N], float top, const Base& k) {
+constexpr int kChunk = 4;  // vectors of a step: 32 or 16 columns
+
+template <typename T>
+__device__ __forceinline__ void soft_absorb(Soft& a, const uint4* v, const Base& k) {
+  constexpr int VN = Elem<T>::kPerVec;
+  float top = Elem<T>::top(v[0]);
+#pragma unroll
+  for (int j = 1; j < kChunk; ++j) top = fmaxf(top, Elem<T>::top(v[j]));
   if (top > a.m) soft_raise(a, top, k);
-  float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
   if (a.m > kLow) {
     const float c = shift_of(a.m, k);
+    const Pair hi2(k.hi, k.hi), c2(c, c);
+    Pair s[2] = {{0.f, 0.f}, {0.f, 0.f}}, t[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = at_least_far(fmaf(x[i], k.hi, c)), e = ex2(d);
-      s[i & 1] += e;
-      t[i & 1] = fmaf(e, d, t[i & 1]);
+    for (int j = 0; j < kChunk; ++j) {
+      float x[VN];
+      Elem<T>::unpack_low(v[j], x);
+#pragma unroll
+      for (int i = 0; i < VN; i += 2) {
+        const Pair d = fma2(Pair(x[i], x[i + 1]), hi2, c2), e = ex2(d);
+        s[(i >> 1) & 1] = add2(s[(i >> 1) & 1], e);
+        t[(i >> 1) & 1] = fma2(e, d, t[(i >> 1) & 1]);
+      }
     }
+    float s0, s1, t0, t1;
+    add2(s[0], s[1]).split(s0, s1);
+    add2(t[0], t[1]).split(t0, t1);
+    a.s += s0 + s1;
+    a.t += t0 + t1;
   } else {
+    float s = 0.f, t = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = at_least_far((x[i] - a.m) * k.hi), e = ex2(d);
-      s[i & 1] += e;
-      t[i & 1] = fmaf(e, d, t[i & 1]);
+    for (int j = 0; j < kChunk; ++j) {
+      float x[VN];
+      Elem<T>::unpack(v[j], x);
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const float d = at_least_far((x[i] - a.m) * k.hi), e = ex2(d);
+        s += e;
+        t = fmaf(e, d, t);
+      }
     }
+    a.s += s;
+    a.t += t;
   }
-  a.s += s[0] + s[1];
-  a.t += t[0] + t[1];
+}
+// One column.
+__device__ __forceinline__ void soft_absorb_one(Soft& a, float x, const Base& k) {
+  if (x > a.m) soft_raise(a, x, k);
+  const float d = at_least_far(a.m > kLow ? fmaf(x, k.hi, shift_of(a.m, k)) : (x - a.m) * k.hi), e = ex2(d);
+  a.s += e;
+  a.t = fmaf(e, d, a.t);
 }
 
 __device__ __forceinline__ void soft_warp_reduce(Soft& a, const Base& k) {
@@ -273,7 +354,7 @@ __device__ __forceinline__ void policy_row(const PolicyTerms& q, const PolicyIn&
 constexpr int kMostThreads = 512;
 constexpr int kMostWarps = kMostThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kFlight = 8;  // 16-byte loads that a thread has in flight
+constexpr int kFlight = 4;  // 16-byte loads that a thread has in flight on the way to the gradient
 
 // A row's columns: up to VN - 1 single ones, 16-byte vectors, up to VN - 1 single ones.
 template <typename T>
@@ -291,38 +372,37 @@ struct RowView {
   }
 };
 
-// This thread's share of the row's sums. Eight loads are issued before the first is used: 128 KB in flight on a
-// multiprocessor of 1,024 threads.
+// The row's single columns, by the first warp of the first CTA.
+template <typename T>
+__device__ __forceinline__ void edge_share(Soft& acc, const T* z, int head, int tail, int64_t vocab, const Base& k) {
+  const int lane = threadIdx.x & 31;
+  if (lane < head) soft_absorb_one(acc, Elem<T>::get(z[lane]), k);
+  if (lane < static_cast<int>(vocab) - tail) soft_absorb_one(acc, Elem<T>::get(z[tail + lane]), k);
+}
+
+// This thread's share of the row's sums. The next vectors are under way while these are summed.
 template <typename T>
 __device__ __forceinline__ Soft row_share(const RowView<T>& r, int64_t vocab, int rank, int ranks, const Base& k) {
-  constexpr int VN = Elem<T>::kPerVec;
-  constexpr int kChunk = 32 / VN;  // vectors of a step: 32 columns
   const int threads = blockDim.x, step = ranks * threads;
   const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
   Soft acc{-FLT_MAX, 0.f, 0.f};
-  for (int i = rank * threads + threadIdx.x; i < r.nvec; i += kFlight * step) {
-    uint4 v[kFlight];
+  int i = rank * threads + threadIdx.x;
+  uint4 v[2][kChunk];
 #pragma unroll
-    for (int j = 0; j < kFlight; ++j) v[j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
+  for (int j = 0; j < kChunk; ++j) v[0][j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
+  while (i < r.nvec) {
 #pragma unroll
-    for (int j = 0; j < kFlight; j += kChunk) {
-      if (j > 0 && i + j * step >= r.nvec) continue;
-      float x[32], top = Elem<T>::top(v[j]);
+    for (int h = 0; h < 2; ++h) {
+      if (i < r.nvec) {
+        const int n = i + kChunk * step;
 #pragma unroll
-      for (int n = 0; n < kChunk; ++n) {
-        Elem<T>::unpack(v[j + n], x + n * VN);
-        top = fmaxf(top, Elem<T>::top(v[j + n]));
+        for (int j = 0; j < kChunk; ++j) v[h ^ 1][j] = n + j * step < r.nvec ? __ldg(r.zv + n + j * step) : none;
+        soft_absorb<T>(acc, v[h], k);
+        i = n;
       }
-      soft_absorb(acc, x, top, k);
     }
   }
-  if (rank == 0 && threadIdx.x < 32 && (r.head > 0 || r.tail < vocab)) {
-    const int lane = threadIdx.x;
-    float x[2] = {-INFINITY, -INFINITY};
-    if (lane < r.head) x[0] = Elem<T>::get(r.z[lane]);
-    if (lane < static_cast<int>(vocab) - r.tail) x[1] = Elem<T>::get(r.z[r.tail + lane]);
-    soft_absorb(acc, x, fmaxf(x[0], x[1]), k);
-  }
+  if (rank == 0 && threadIdx.x < 32) edge_share(acc, r.z, r.head, r.tail, vocab, k);
   return acc;
 }
 
@@ -375,14 +455,17 @@ struct RowGrad {
   __device__ __forceinline__ uint4 vec(const uint4& v, int col, int tok) const {
     constexpr int VN = Elem<T>::kPerVec;
     float x[VN];
-    Elem<T>::unpack(v, x);
     if (cf.y > 0.f) {
+      if (kEnt) Elem<T>::unpack_low(v, x);
+      else Elem<T>::unpack(v, x);
+      const Pair hi2(hi, hi), cx(cf.x, cf.x), c02(c0, c0), c12(c1, c1);
 #pragma unroll
-      for (int e = 0; e < VN; ++e) {
-        const float q = fmaf(x[e], hi, cf.x);
-        x[e] = ex2(q) * (kEnt ? fmaf(c1, fmaxf(q, kFar), c0) : c0);
+      for (int e = 0; e < VN; e += 2) {
+        const Pair q = fma2(Pair(x[e], x[e + 1]), hi2, cx);
+        mul2(ex2(q), kEnt ? fma2(c12, q, c02) : c02).split(x[e], x[e + 1]);
       }
     } else {
+      Elem<T>::unpack(v, x);
 #pragma unroll
       for (int e = 0; e < VN; ++e) x[e] = this->template operator()<kEnt>(x[e]);
     }
@@ -400,10 +483,9 @@ struct RowGrad {
 };
 
 template <typename T>
-__device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ranks) {
+__device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ranks, int threads) {
   const RowView<T> r(out, vocab);
   uint4* ov = reinterpret_cast<uint4*>(out + r.head);
-  const int threads = blockDim.x;
   for (int i = rank * threads + threadIdx.x; i < r.nvec; i += ranks * threads) __stcs(ov + i, make_uint4(0, 0, 0, 0));
   if (rank == 0 && static_cast<int>(threadIdx.x) < r.head) out[threadIdx.x] = Elem<T>::put(0.f);
   if (rank == 0 && static_cast<int>(threadIdx.x) < static_cast<int>(vocab) - r.tail) {
@@ -501,7 +583,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_policy_kernel(const Tok
         a.logp[row] = 0.f;
         a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      zero_row(out, a.vocab, rank, ranks);
+      zero_row(out, a.vocab, rank, ranks, threads);
       continue;
     }
     const RowView<T> r(row_ptr<const T>(a.z, row), a.vocab);
@@ -526,7 +608,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_policy_kernel(const Tok
     const RowGrad g = s_grad[parity];
     parity ^= 1;
     if (g.a == 0.f && (!kEnt || g.c1 == 0.f)) {
-      zero_row(out, a.vocab, rank, ranks);
+      zero_row(out, a.vocab, rank, ranks, threads);
       continue;
     }
     uint4* ov = reinterpret_cast<uint4*>(out + r.head);
@@ -564,6 +646,8 @@ constexpr int kStages = 3;
 struct RingItem {  // one row of a stage
   int64_t row;     // -1: no more rows
   int tok;         // -1: the row does not count
+  int count, col;  // vectors of the slice, column of the first
+  int head, tail;  // the row's single columns: before `head` and from `tail` on
   float w, zt, old_logp, adv, ref_logp;
 };
 struct RingShared {
@@ -660,7 +744,11 @@ __device__ __forceinline__ void ring_move(const TokenStatsArgs& a, const PolicyT
     if (it.tok < 0) return it;
     const PolicyIn in(q, r);
     it.old_logp = in.old_logp, it.adv = in.adv, it.ref_logp = in.ref_logp;
-    it.zt = Elem<T>::get(row_ptr<const T>(a.z, r)[it.tok]);
+    const RowView<T> v(row_ptr<const T>(a.z, r), a.vocab);
+    const Slice<T> sl(v, rank, ranks);
+    it.count = sl.v1 - sl.v0, it.col = v.head + sl.v0 * Elem<T>::kPerVec;
+    it.head = v.head, it.tail = v.tail;
+    it.zt = Elem<T>::get(v.z[it.tok]);
     return it;
   };
   auto publish = [&](int s, const RingItem& it) {
@@ -669,11 +757,9 @@ __device__ __forceinline__ void ring_move(const TokenStatsArgs& a, const PolicyT
       mbar_arrive(&sh.full[s]);
       return;
     }
-    const RowView<T> r(row_ptr<const T>(a.z, it.row), a.vocab);
-    const Slice<T> sl(r, rank, ranks);
-    const uint32_t bytes = static_cast<uint32_t>(sl.v1 - sl.v0) * 16u;
+    const uint32_t bytes = static_cast<uint32_t>(it.count) * 16u;
     mbar_arrive_expect_tx(&sh.full[s], bytes);
-    if (bytes) bulk_load(ring + s * stage_bytes, r.zv + sl.v0, bytes, &sh.full[s]);
+    if (bytes) bulk_load(ring + s * stage_bytes, row_ptr<const T>(a.z, it.row) + it.col, bytes, &sh.full[s]);
   };
   for (int s = 0; s < kStages; ++s, row += row_step) publish(s, look(row));
   for (RingCursor c;; c.next(), row += row_step) {
@@ -686,12 +772,8 @@ __device__ __forceinline__ void ring_move(const TokenStatsArgs& a, const PolicyT
       break;
     }
     if (it.tok >= 0) {
-      T* out = row_ptr<T>(grad, it.row);
-      const RowView<T> r(out, a.vocab);
-      const Slice<T> sl(r, rank, ranks);
-      if (sl.v1 > sl.v0) {
-        bulk_store(out + r.head + static_cast<int64_t>(sl.v0) * Elem<T>::kPerVec, ring + c.stage * stage_bytes,
-                   static_cast<uint32_t>(sl.v1 - sl.v0) * 16u);
+      if (it.count) {
+        bulk_store(row_ptr<T>(grad, it.row) + it.col, ring + c.stage * stage_bytes, static_cast<uint32_t>(it.count) * 16u);
       }
       bulk_commit_group();
       bulk_wait_group_read<0>();
@@ -771,33 +853,20 @@ template <typename T, bool kEnt>
 __device__ __forceinline__ void ring_compute(const TokenStatsArgs& a, const TokenRows& grad, const Base& k,
                                              RingShared& sh, uint8_t* ring, int stage_bytes, int rank, int ranks) {
   constexpr int VN = Elem<T>::kPerVec;
-  constexpr int kChunk = 32 / VN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
 
   auto sum = [&](int stage, const RingItem& it, int b) {
-    const RowView<T> r(row_ptr<const T>(a.z, it.row), a.vocab);
-    const Slice<T> sl(r, rank, ranks);
-    const int count = sl.v1 - sl.v0;
     const uint4* v = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
     Soft acc{-FLT_MAX, 0.f, 0.f};
-    for (int i = threadIdx.x; i < count; i += kChunk * kRingThreads) {
+    for (int i = threadIdx.x; i < it.count; i += kChunk * kRingThreads) {
       uint4 c[kChunk];
 #pragma unroll
-      for (int j = 0; j < kChunk; ++j) c[j] = i + j * kRingThreads < count ? v[i + j * kRingThreads] : none;
-      float x[32], top = Elem<T>::top(c[0]);
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j) {
-        Elem<T>::unpack(c[j], x + j * VN);
-        top = fmaxf(top, Elem<T>::top(c[j]));
-      }
-      soft_absorb(acc, x, top, k);
+      for (int j = 0; j < kChunk; ++j) c[j] = i + j * kRingThreads < it.count ? v[i + j * kRingThreads] : none;
+      soft_absorb<T>(acc, c, k);
     }
-    if (rank == 0 && warp == 0 && (r.head > 0 || r.tail < a.vocab)) {  // columns before and behind the vectors
-      float x[2] = {-INFINITY, -INFINITY};
-      if (lane < r.head) x[0] = Elem<T>::get(r.z[lane]);
-      if (lane < static_cast<int>(a.vocab) - r.tail) x[1] = Elem<T>::get(r.z[r.tail + lane]);
-      soft_absorb(acc, x, fmaxf(x[0], x[1]), k);
+    if (rank == 0 && warp == 0 && (it.head > 0 || it.tail < a.vocab)) {
+      edge_share(acc, row_ptr<const T>(a.z, it.row), it.head, it.tail, a.vocab, k);
     }
     soft_warp_reduce(acc, k);
     if (lane == 0) {
@@ -807,38 +876,31 @@ __device__ __forceinline__ void ring_compute(const TokenStatsArgs& a, const Toke
   };
 
   auto turn = [&](int stage, const RingItem& it, int b) {
-    T* out = row_ptr<T>(grad, it.row);
-    const RowView<T> r(out, a.vocab);  // starts where the logits' row does within 16 bytes
-    const Slice<T> sl(r, rank, ranks);
-    const int count = sl.v1 - sl.v0;
-    const int end = r.tail + static_cast<int>(threadIdx.x);
-    const bool before = rank == 0 && static_cast<int>(threadIdx.x) < r.head;
-    const bool behind = rank == 0 && end < static_cast<int>(a.vocab);
     if (it.tok < 0) {
-      uint4* ov = reinterpret_cast<uint4*>(out + r.head) + sl.v0;
-      for (int i = threadIdx.x; i < count; i += kRingThreads) __stcs(ov + i, make_uint4(0, 0, 0, 0));
-      if (before) out[threadIdx.x] = Elem<T>::put(0.f);
-      if (behind) out[end] = Elem<T>::put(0.f);
+      zero_row(row_ptr<T>(grad, it.row), a.vocab, rank, ranks, kRingThreads);
       return;
     }
     const RowGrad g = sh.grad[b];
     uint4* v = reinterpret_cast<uint4*>(ring + stage * stage_bytes);
-    const int col = r.head + sl.v0 * VN;
-    for (int i = threadIdx.x; i < count; i += 4 * kRingThreads) {
+    for (int i = threadIdx.x; i < it.count; i += 4 * kRingThreads) {
       uint4 c[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (i + j * kRingThreads < count) c[j] = v[i + j * kRingThreads];
+        if (i + j * kRingThreads < it.count) c[j] = v[i + j * kRingThreads];
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = i + j * kRingThreads;
-        if (at < count) v[at] = g.template vec<T, kEnt>(c[j], col + at * VN, it.tok);
+        if (at < it.count) v[at] = g.template vec<T, kEnt>(c[j], it.col + at * VN, it.tok);
       }
     }
-    const T* z = row_ptr<const T>(a.z, it.row);
-    if (before) out[threadIdx.x] = g.template one<T, kEnt>(z[threadIdx.x], threadIdx.x, it.tok);
-    if (behind) out[end] = g.template one<T, kEnt>(z[end], end, it.tok);
+    if (rank == 0 && warp == 0 && (it.head > 0 || it.tail < a.vocab)) {
+      const T* z = row_ptr<const T>(a.z, it.row);
+      T* out = row_ptr<T>(grad, it.row);
+      if (lane < it.head) out[lane] = g.template one<T, kEnt>(z[lane], lane, it.tok);
+      const int end = it.tail + lane;
+      if (end < static_cast<int>(a.vocab)) out[end] = g.template one<T, kEnt>(z[end], end, it.tok);
+    }
     fence_proxy_async_smem();
   };
 
