@@ -351,7 +351,7 @@ __device__ __forceinline__ void policy_row(const PolicyTerms& q, const PolicyIn&
 }
 
 // ---- a row per CTA or cluster -------------------------------------------------------------------------------------------
-constexpr int kMostThreads = 512;
+constexpr int kMostThreads = 256;
 constexpr int kMostWarps = kMostThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kFlight = 4;  // 16-byte loads that a thread has in flight on the way to the gradient
@@ -380,27 +380,19 @@ __device__ __forceinline__ void edge_share(Soft& acc, const T* z, int head, int 
   if (lane < static_cast<int>(vocab) - tail) soft_absorb_one(acc, Elem<T>::get(z[tail + lane]), k);
 }
 
-// This thread's share of the row's sums. The next vectors are under way while these are summed.
+// This thread's share of the row's sums. Eight loads are issued before the first is used: 128 KB in flight on a
+// multiprocessor of 1,024 threads.
 template <typename T>
 __device__ __forceinline__ Soft row_share(const RowView<T>& r, int64_t vocab, int rank, int ranks, const Base& k) {
   const int threads = blockDim.x, step = ranks * threads;
   const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
   Soft acc{-FLT_MAX, 0.f, 0.f};
-  int i = rank * threads + threadIdx.x;
-  uint4 v[2][kChunk];
+  for (int i = rank * threads + threadIdx.x; i < r.nvec; i += 2 * kChunk * step) {
+    uint4 v[2 * kChunk];
 #pragma unroll
-  for (int j = 0; j < kChunk; ++j) v[0][j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
-  while (i < r.nvec) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (i < r.nvec) {
-        const int n = i + kChunk * step;
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[h ^ 1][j] = n + j * step < r.nvec ? __ldg(r.zv + n + j * step) : none;
-        soft_absorb<T>(acc, v[h], k);
-        i = n;
-      }
-    }
+    for (int j = 0; j < 2 * kChunk; ++j) v[j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
+    soft_absorb<T>(acc, v, k);
+    if (i + kChunk * step < r.nvec) soft_absorb<T>(acc, v + kChunk, k);
   }
   if (rank == 0 && threadIdx.x < 32) edge_share(acc, r.z, r.head, r.tail, vocab, k);
   return acc;
@@ -497,7 +489,7 @@ __device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ra
 // A CTA per row, or a cluster of them where rows are few: each CTA a share of the row's vectors, whose sums meet in every
 // CTA's shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kMostThreads, 2) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
+__global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                       bool policy, const Base k) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
@@ -548,7 +540,7 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem);
 // A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
 // the rows in work fit L2 (row_ranks), so the logits come from memory once.
 template <typename T, bool kEnt>
-__global__ void __launch_bounds__(kMostThreads, 2) token_policy_kernel(const TokenStatsArgs a, const PolicyTerms q,
+__global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                        const TokenRows grad, float scale,
                                                                        const float* scale_device, int mean,
                                                                        const Base k) {
@@ -1050,7 +1042,7 @@ cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// Threads of a CTA: eight vectors each, 32 to 512. CTAs of a row: as many as leave every thread a vector while all rows
+// Threads of a CTA: eight vectors each, 32 to 256. CTAs of a row: as many as leave every thread a vector while all rows
 // together stay within one wave; and with `again` (the row is read a second time) as many as keep the rows of a wave
 // within `kCached` bytes.
 constexpr int64_t kCached = 80 << 20;
