@@ -177,7 +177,8 @@ Tensor token_logprobs_backward(const Tensor& logits, const Tensor& tokens, const
 }
 
 // ---- policy loss ------------------------------------------------------------------------------------------------------
-// Returns [out (6), logp, grad] with want_grad, [out (6), logp, entropy, ml, coef] without.
+// Returns loss, surrogate, kl, entropy mean, clip fraction, factor, logp, then [grad] with want_grad, [entropy, ml, coef]
+// without.
 std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logp,
                                       const Tensor& advantages, const OptT& ref_logp, const OptT& mask, double clip_lo,
                                       double clip_hi, double kl_coef, int64_t kl_kind, double entropy_coef,
@@ -200,7 +201,7 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   q.clip_lo = static_cast<float>(clip_lo), q.clip_hi = static_cast<float>(clip_hi);
   q.kl_coef = static_cast<float>(kl_coef), q.entropy_coef = static_cast<float>(entropy_coef);
   q.kl_kind = static_cast<int>(kl_kind);
-  Tensor out = torch::empty({6}, l.f32()), logp = torch::empty(l.lead(), l.f32());
+  Tensor loss = torch::empty({}, l.f32()), out = torch::empty({5}, l.f32()), logp = torch::empty(l.lead(), l.f32());
   Tensor terms = torch::empty({l.rows, 4}, l.f32()), entropy, ml, coef, grad;
   if (want_grad) grad = l.gradient();
   const bool one_pass = want_grad && l.same_phase(grad);
@@ -223,9 +224,15 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   }
   rlb::PolicyFinishArgs f{};
   f.rows = l.rows, f.terms = a.terms, f.idx = ix.idx, f.vocab = l.vocab, f.kl_coef = q.kl_coef;
-  f.entropy_coef = q.entropy_coef, f.mean = mean, f.out = out.data_ptr<float>();
+  f.entropy_coef = q.entropy_coef, f.mean = mean, f.loss = loss.data_ptr<float>(), f.out = out.data_ptr<float>();
   ok(rlb::policy_finish(f, stream), "token_policy_loss");
-  if (!want_grad) return {out, logp, entropy, ml, coef};
+  std::vector<Tensor> result = out.unbind();
+  result.insert(result.begin(), loss);
+  result.push_back(logp);
+  if (!want_grad) {
+    result.insert(result.end(), {entropy, ml, coef});
+    return result;
+  }
   if (!one_pass) {
     rlb::TokenGradArgs g{};
     g.dtype = l.dtype, g.rows = l.rows, g.vocab = l.vocab, g.z = l.z, g.idx = ix.idx, g.inv_temp = a.inv_temp;
@@ -235,10 +242,11 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
     if (q.entropy_coef != 0.f) g.b = coef.data_ptr<float>() + 1, g.b_stride = 2;
     g.weighted = 1;
     g.scale = static_cast<float>(grad_scale), g.scale_a = scale_device;
-    g.scale_b = out.data_ptr<float>() + 5;
+    g.scale_b = out.data_ptr<float>() + 4;
     ok(rlb::token_grad(g, stream), "token_policy_loss");
   }
-  return {out, logp, grad};
+  result.push_back(grad);
+  return result;
 }
 
 // Gradient from what token_policy_loss returned without its gradient (or preference_loss, with factor and entropy unset).

@@ -71,6 +71,27 @@ __device__ __forceinline__ float at_least_low(float z) {  // a NaN stays one
   return y;
 }
 
+// Loads of a row that is read twice: the first keeps it in L2, the second lets it go.
+__device__ __forceinline__ uint4 load_hint(const uint4* p, uint64_t policy) {
+  uint4 v;
+  asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p), "l"(policy));
+  return v;
+}
+template <bool kAgain>
+__device__ __forceinline__ uint4 load_first(const uint4* p) {
+  if (!kAgain) return __ldg(p);
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+  return load_hint(p, policy);
+}
+__device__ __forceinline__ uint4 load_last(const uint4* p) {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return load_hint(p, policy);
+}
+
 template <typename T>
 struct Elem;
 template <>
@@ -382,7 +403,7 @@ __device__ __forceinline__ void edge_share(Soft& acc, const T* z, int head, int 
 
 // This thread's share of the row's sums. Eight loads are issued before the first is used: 128 KB in flight on a
 // multiprocessor of 1,024 threads.
-template <typename T>
+template <bool kAgain, typename T>
 __device__ __forceinline__ Soft row_share(const RowView<T>& r, int64_t vocab, int rank, int ranks, const Base& k) {
   const int threads = blockDim.x, step = ranks * threads;
   const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
@@ -390,7 +411,7 @@ __device__ __forceinline__ Soft row_share(const RowView<T>& r, int64_t vocab, in
   for (int i = rank * threads + threadIdx.x; i < r.nvec; i += 2 * kChunk * step) {
     uint4 v[2 * kChunk];
 #pragma unroll
-    for (int j = 0; j < 2 * kChunk; ++j) v[j] = i + j * step < r.nvec ? __ldg(r.zv + i + j * step) : none;
+    for (int j = 0; j < 2 * kChunk; ++j) v[j] = i + j * step < r.nvec ? load_first<kAgain>(r.zv + i + j * step) : none;
     soft_absorb<T>(acc, v, k);
     if (i + kChunk * step < r.nvec) soft_absorb<T>(acc, v + kChunk, k);
   }
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const Toke
     }
     const RowView<T> r(row_ptr<const T>(a.z, row), a.vocab);
     const float zt = Elem<T>::get(r.z[tok]);
-    const Soft acc = row_total(row_share(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
+    const Soft acc = row_total(row_share<false>(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
     parity ^= 1;
     if (rank == 0 && threadIdx.x == 0) {
       const RowSoft soft = row_soft(acc, k);
@@ -581,7 +602,7 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
     const RowView<T> r(row_ptr<const T>(a.z, row), a.vocab);
     const PolicyIn in(q, row);
     const float zt = Elem<T>::get(r.z[tok]);
-    const Soft acc = row_total(row_share(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
+    const Soft acc = row_total(row_share<true>(r, a.vocab, rank, ranks, k), x, parity, rank, ranks, k, cluster);
     if (threadIdx.x < 32) {
       const RowSoft soft = row_soft(acc, k);
       const float logp = row_logp(soft, zt, k);
@@ -609,7 +630,7 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
       uint4 v[kFlight];
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (i + j * step < r.nvec) v[j] = __ldg(r.zv + i + j * step);
+        if (i + j * step < r.nvec) v[j] = load_last(r.zv + i + j * step);
       }
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
@@ -623,339 +644,6 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
     const int end = r.tail + static_cast<int>(threadIdx.x);
     if (rank == 0 && end < static_cast<int>(a.vocab)) out[end] = g.template one<T, kEnt>(r.z[end], end, tok);
   }
-}
-
-// ---- the same with the row in shared memory ------------------------------------------------------------------------------
-// A cluster of CTAs holds a row, each CTA a slice of it. Eight warps turn slices into their gradients in place; one warp
-// moves slices, by bulk copies into a ring of stages and out of them; one warp does what a row needs once: it joins the
-// sums, exchanges them with the other CTAs and works out the coefficients. The eight warps sum row n + 1 before they turn
-// to the gradient of row n, which gives the exchange the time of a row. The logits are read once and the gradient written
-// once, both without registers.
-constexpr int kRingWarps = 8;
-constexpr int kRingThreads = kRingWarps * 32;  // that compute
-constexpr int kStages = 3;
-
-struct RingItem {  // one row of a stage
-  int64_t row;     // -1: no more rows
-  int tok;         // -1: the row does not count
-  int count, col;  // vectors of the slice, column of the first
-  int head, tail;  // the row's single columns: before `head` and from `tail` on
-  float w, zt, old_logp, adv, ref_logp;
-};
-struct RingShared {
-  uint64_t full[kStages], done[kStages];  // a stage's slice has arrived / has been used
-  uint64_t summed[2], met[2], ready[2];   // a row's sums: of the warps, of the CTAs; its coefficients
-  RingItem item[kStages];
-  Soft warp[2][kRingWarps];
-  float4 cta[2][kMaxCluster];
-  RowGrad grad[2];
-  int lost;  // a wait ran out of time: nothing waits any more, the losses become NaN
-};
-
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ uint32_t peer_address(const void* p, int rank) {
-  uint32_t y;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(smem_u32(p)), "r"(rank));
-  return y;
-}
-// Puts v into a peer's slot and arrives at the peer's barrier.
-__device__ __forceinline__ void peer_put(uint32_t slot, uint32_t bar, const Soft& v) {
-  asm volatile(
-      "st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %3};\n\t"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%4];\n" ::"r"(slot),
-      "f"(v.m), "f"(v.s), "f"(v.t), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ bool peer_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Waits for a phase, at most kWaitTimeoutNs, and not at all once a wait has failed.
-__device__ __forceinline__ void ring_wait(RingShared& sh, uint64_t* bar, uint32_t parity) {
-  if (peer_try_wait(bar, parity)) return;
-  const uint64_t t0 = globaltimer_ns();
-  while (!peer_try_wait(bar, parity)) {
-    if (*const_cast<volatile int*>(&sh.lost) || globaltimer_ns() - t0 > kWaitTimeoutNs) {
-      *const_cast<volatile int*>(&sh.lost) = 1;
-      return;
-    }
-  }
-}
-// The same answer in every lane.
-__device__ __forceinline__ bool ring_lost(const RingShared& sh) {
-  return __any_sync(__activemask(), *const_cast<volatile const int*>(&sh.lost) != 0);
-}
-
-template <typename T>
-struct Slice {  // this CTA's vectors of a row
-  int v0, v1;
-  __device__ __forceinline__ Slice(const RowView<T>& r, int rank, int ranks) {
-    const int shift = 31 - __clz(ranks);                         // ranks are a power of two
-    const int per = (((r.nvec + ranks - 1) >> shift) + 7) & ~7;  // whole 128-byte lines
-    v0 = min(rank * per, r.nvec);
-    v1 = min(v0 + per, r.nvec);
-  }
-};
-
-struct RingCursor {  // walks the stages of the ring
-  int stage = 0;
-  uint32_t parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++stage == kStages) stage = 0, parity ^= 1u;
-  }
-};
-
-// The mover: one thread. It looks rows up stages ahead of the arithmetic, starts their copies, and sends gradients off.
-template <typename T>
-__device__ __forceinline__ void ring_move(const TokenStatsArgs& a, const PolicyTerms& q, const TokenRows& grad,
-                                          RingShared& sh, uint8_t* ring, int stage_bytes, int rank, int ranks) {
-  const int64_t row_step = gridDim.x / ranks;
-  int64_t row = blockIdx.x / ranks;
-  auto look = [&](int64_t r) {
-    RingItem it;
-    it.row = r < a.rows ? r : -1;
-    it.tok = -1;
-    if (it.row < 0) return it;
-    it.tok = static_cast<int>(row_token(a.idx, r, a.vocab, it.w));
-    if (it.tok < 0) return it;
-    const PolicyIn in(q, r);
-    it.old_logp = in.old_logp, it.adv = in.adv, it.ref_logp = in.ref_logp;
-    const RowView<T> v(row_ptr<const T>(a.z, r), a.vocab);
-    const Slice<T> sl(v, rank, ranks);
-    it.count = sl.v1 - sl.v0, it.col = v.head + sl.v0 * Elem<T>::kPerVec;
-    it.head = v.head, it.tail = v.tail;
-    it.zt = Elem<T>::get(v.z[it.tok]);
-    return it;
-  };
-  auto publish = [&](int s, const RingItem& it) {
-    sh.item[s] = it;
-    if (it.tok < 0) {
-      mbar_arrive(&sh.full[s]);
-      return;
-    }
-    const uint32_t bytes = static_cast<uint32_t>(it.count) * 16u;
-    mbar_arrive_expect_tx(&sh.full[s], bytes);
-    if (bytes) bulk_load(ring + s * stage_bytes, row_ptr<const T>(a.z, it.row) + it.col, bytes, &sh.full[s]);
-  };
-  for (int s = 0; s < kStages; ++s, row += row_step) publish(s, look(row));
-  for (RingCursor c;; c.next(), row += row_step) {
-    const RingItem next = look(row);
-    const RingItem it = sh.item[c.stage];
-    if (it.row < 0) break;
-    ring_wait(sh, &sh.done[c.stage], c.parity);
-    if (ring_lost(sh)) {  // no more copies; those under way end before the memory does
-      for (int s = 0; s < kStages; ++s, c.next()) mbar_wait(&sh.full[c.stage], c.parity);
-      break;
-    }
-    if (it.tok >= 0) {
-      if (it.count) {
-        bulk_store(row_ptr<T>(grad, it.row) + it.col, ring + c.stage * stage_bytes, static_cast<uint32_t>(it.count) * 16u);
-      }
-      bulk_commit_group();
-      bulk_wait_group_read<0>();
-    }
-    publish(c.stage, next);
-  }
-}
-
-// What a row needs once: one warp.
-template <typename T, bool kEnt>
-__device__ __forceinline__ void ring_join(const TokenStatsArgs& a, const PolicyTerms& q, float scale,
-                                          const float* scale_device, int mean, const Base& k, RingShared& sh, int rank,
-                                          int ranks) {
-  const int lane = threadIdx.x & 31;
-  if (scale_device) scale *= *scale_device;
-  if (mean) {  // every CTA sums the weights for itself, in the same order
-    double total = 0.0;
-    for (int64_t r = lane; r < a.rows; r += 32) {
-      float w;
-      row_token(a.idx, r, a.vocab, w);
-      total += w;
-    }
-    for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    scale *= total != 0.0 ? static_cast<float>(1.0 / total) : 0.f;
-  }
-  const float factor = scale * k.inv;
-  uint32_t rounds = 0;
-  for (RingCursor c;; c.next()) {
-    ring_wait(sh, &sh.full[c.stage], c.parity);
-    if (ring_lost(sh)) break;
-    const RingItem it = sh.item[c.stage];
-    if (it.row < 0) break;
-    if (it.tok < 0) {
-      if (rank == 0 && lane == 0) {
-        a.logp[it.row] = 0.f;
-        a.terms[it.row] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.done[c.stage]);
-      continue;
-    }
-    const int b = rounds & 1;
-    const uint32_t phase = (rounds >> 1) & 1;
-    ++rounds;
-    ring_wait(sh, &sh.summed[b], phase);
-    Soft acc = lane < kRingWarps ? sh.warp[b][lane] : Soft{-FLT_MAX, 0.f, 0.f};
-    soft_warp_reduce(acc, k);
-    if (ranks > 1) {
-      // a slot is free: a peer that sends its sums of this row has read those of the row before last
-      if (lane < ranks) peer_put(peer_address(&sh.cta[b][rank], lane), peer_address(&sh.met[b], lane), acc);
-      ring_wait(sh, &sh.met[b], phase);
-      const float4 p = sh.cta[b][lane < ranks ? lane : 0];
-      acc = lane < ranks ? Soft{p.x, p.y, p.z} : Soft{-FLT_MAX, 0.f, 0.f};
-      soft_warp_reduce(acc, k);
-    }
-    const RowSoft soft = row_soft(acc, k);
-    const float logp = row_logp(soft, it.zt, k);
-    float4 terms;
-    float2 coef;
-    policy_row(q, PolicyIn(it.old_logp, it.adv, it.ref_logp), logp, soft.entropy, it.w, terms, coef);
-    const RowGrad g(row_shift(soft, k), k, coef.x * factor, kEnt ? coef.y * factor : 0.f, soft.entropy);
-    if (ring_lost(sh)) terms.x = __int_as_float(0x7fffffff);
-    if (lane == 0) {
-      sh.grad[b] = g;
-      mbar_arrive(&sh.ready[b]);
-      mbar_arrive(&sh.done[c.stage]);
-      if (rank == 0) {
-        a.logp[it.row] = logp;
-        a.terms[it.row] = terms;
-      }
-    }
-  }
-}
-
-// The arithmetic: eight warps.
-template <typename T, bool kEnt>
-__device__ __forceinline__ void ring_compute(const TokenStatsArgs& a, const TokenRows& grad, const Base& k,
-                                             RingShared& sh, uint8_t* ring, int stage_bytes, int rank, int ranks) {
-  constexpr int VN = Elem<T>::kPerVec;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint4 none = make_uint4(Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone, Elem<T>::kNone);
-
-  auto sum = [&](int stage, const RingItem& it, int b) {
-    const uint4* v = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
-    Soft acc{-FLT_MAX, 0.f, 0.f};
-    for (int i = threadIdx.x; i < it.count; i += kChunk * kRingThreads) {
-      uint4 c[kChunk];
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j) c[j] = i + j * kRingThreads < it.count ? v[i + j * kRingThreads] : none;
-      soft_absorb<T>(acc, c, k);
-    }
-    if (rank == 0 && warp == 0 && (it.head > 0 || it.tail < a.vocab)) {
-      edge_share(acc, row_ptr<const T>(a.z, it.row), it.head, it.tail, a.vocab, k);
-    }
-    soft_warp_reduce(acc, k);
-    if (lane == 0) {
-      sh.warp[b][warp] = acc;
-      mbar_arrive(&sh.summed[b]);
-    }
-  };
-
-  auto turn = [&](int stage, const RingItem& it, int b) {
-    if (it.tok < 0) {
-      zero_row(row_ptr<T>(grad, it.row), a.vocab, rank, ranks, kRingThreads);
-      return;
-    }
-    const RowGrad g = sh.grad[b];
-    uint4* v = reinterpret_cast<uint4*>(ring + stage * stage_bytes);
-    for (int i = threadIdx.x; i < it.count; i += 4 * kRingThreads) {
-      uint4 c[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j * kRingThreads < it.count) c[j] = v[i + j * kRingThreads];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = i + j * kRingThreads;
-        if (at < it.count) v[at] = g.template vec<T, kEnt>(c[j], it.col + at * VN, it.tok);
-      }
-    }
-    if (rank == 0 && warp == 0 && (it.head > 0 || it.tail < a.vocab)) {
-      const T* z = row_ptr<const T>(a.z, it.row);
-      T* out = row_ptr<T>(grad, it.row);
-      if (lane < it.head) out[lane] = g.template one<T, kEnt>(z[lane], lane, it.tok);
-      const int end = it.tail + lane;
-      if (end < static_cast<int>(a.vocab)) out[end] = g.template one<T, kEnt>(z[end], end, it.tok);
-    }
-    fence_proxy_async_smem();
-  };
-
-  RingCursor ahead, here;
-  uint32_t sums = 0, turns = 0;
-  RingItem now, next;
-  auto fetch = [&](RingItem& it) {  // the item ahead, and its sums
-    ring_wait(sh, &sh.full[ahead.stage], ahead.parity);
-    it = sh.item[ahead.stage];
-    if (ring_lost(sh)) it.row = -1;
-    if (it.row >= 0 && it.tok >= 0) sum(ahead.stage, it, sums++ & 1);
-    if (it.row >= 0) ahead.next();
-  };
-  fetch(now);
-  while (now.row >= 0) {
-    fetch(next);
-    const int b = turns & 1;
-    if (now.tok >= 0) {
-      ring_wait(sh, &sh.ready[b], (turns >> 1) & 1);
-      ++turns;
-    }
-    if (ring_lost(sh)) break;
-    turn(here.stage, now, b);
-    mbar_arrive(&sh.done[here.stage]);
-    here.next();
-    now = next;
-  }
-}
-
-template <typename T, bool kEnt>
-__global__ void __launch_bounds__(kRingThreads + 64, 2) token_policy_ring_kernel(
-    const TokenStatsArgs a, const PolicyTerms q, const TokenRows grad, float scale, const float* scale_device, int mean,
-    const Base k, int stage_bytes) {
-  griddep_wait();  // launched with programmatic stream serialization
-  griddep_launch_dependents();
-  extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ RingShared sh;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sh.full[s], 1);
-      mbar_init(&sh.done[s], kRingThreads + 1);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&sh.summed[b], kRingWarps);
-      mbar_init(&sh.met[b], ranks);
-      mbar_init(&sh.ready[b], 1);
-    }
-    sh.lost = 0;
-    fence_mbar_init();
-  }
-  cluster.sync();  // the barriers of every CTA are ready
-  const int warp = threadIdx.x >> 5;
-  if (warp < kRingWarps) {
-    ring_compute<T, kEnt>(a, grad, k, sh, ring, stage_bytes, rank, ranks);
-  } else if (warp == kRingWarps) {
-    ring_join<T, kEnt>(a, q, scale, scale_device, mean, k, sh, rank, ranks);
-  } else {
-    if ((threadIdx.x & 31) == 0) ring_move<T>(a, q, grad, sh, ring, stage_bytes, rank, ranks);
-    __syncwarp();
-  }
-  cluster.sync();  // no CTA leaves while another may still write into it
 }
 
 int sm_count() {
@@ -975,21 +663,15 @@ Base base_of(double inv_temp) {
   return b;
 }
 
-// Rows from 8 KB up to 8 slices of 72 KB go through shared memory: slices of at most 32 KB where eight CTAs can hold the row
-// that way (two CTAs a multiprocessor), else of at most 72 KB (one).
-constexpr int64_t kRingLeast = 8 << 10, kRingSlice = 32 << 10, kRingMost = 72 << 10;
-
 struct RowLaunch {
   int threads, ranks;
   int64_t clusters;
-  int smem = 0;
 };
 
 cudaLaunchConfig_t row_config(const RowLaunch& l, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.clusters * l.ranks));
   cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(l.smem);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(l.ranks);
@@ -1007,7 +689,7 @@ template <typename Kern>
 cudaError_t resident_clusters(Kern kern, const RowLaunch& l, int* count) {
   struct Known {
     const void* kern;
-    int device, ranks, smem, count;
+    int device, ranks, threads, count;
   };
   static std::mutex lock;
   static std::vector<Known> known;
@@ -1016,13 +698,11 @@ cudaError_t resident_clusters(Kern kern, const RowLaunch& l, int* count) {
   if (e != cudaSuccess) return e;
   const std::lock_guard<std::mutex> guard(lock);
   for (const Known& x : known) {
-    if (x.kern == reinterpret_cast<const void*>(kern) && x.device == device && x.ranks == l.ranks && x.smem == l.smem) {
+    if (x.kern == reinterpret_cast<const void*>(kern) && x.device == device && x.ranks == l.ranks && x.threads == l.threads) {
       *count = x.count;
       return cudaSuccess;
     }
   }
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kRingMost) * kStages);
-  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   RowLaunch one = l;
   one.clusters = 1;
@@ -1031,7 +711,7 @@ cudaError_t resident_clusters(Kern kern, const RowLaunch& l, int* count) {
   e = cudaOccupancyMaxActiveClusters(count, kern, &cfg);
   if (e != cudaSuccess) return e;
   *count = std::max(*count, 1);
-  known.push_back({reinterpret_cast<const void*>(kern), device, l.ranks, l.smem, *count});
+  known.push_back({reinterpret_cast<const void*>(kern), device, l.ranks, l.threads, *count});
   return cudaSuccess;
 }
 
@@ -1046,7 +726,7 @@ cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t
 // together stay within one wave; and with `again` (the row is read a second time) as many as keep the rows of a wave
 // within `kCached` bytes.
 constexpr int64_t kCached = 80 << 20;
-RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again, int waves) {
+RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again) {
   const int64_t sms = sm_count(), nvec = vocab * size / 16;
   RowLaunch l;
   l.threads = static_cast<int>(std::min<int64_t>(kMostThreads, std::max<int64_t>(32, (nvec / 8 + 31) / 32 * 32)));
@@ -1058,7 +738,7 @@ RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again, int wave
     if (!idle && !large) break;
     l.ranks *= 2;
   }
-  l.clusters = std::max<int64_t>(1, std::min(rows, waves * resident / l.ranks));
+  l.clusters = std::min(rows, 32 * resident / l.ranks);
   return l;
 }
 
@@ -1066,7 +746,7 @@ template <typename T>
 cudaError_t launch_stats(const TokenStatsArgs& a, cudaStream_t stream) {
   PolicyTerms q{};
   if (a.policy) q = *a.policy;
-  return launch_rows(token_stats_kernel<T>, row_launch(a.rows, a.vocab, sizeof(T), false, 32), stream, a, q,
+  return launch_rows(token_stats_kernel<T>, row_launch(a.rows, a.vocab, sizeof(T), false), stream, a, q,
                      a.policy != nullptr, base_of(a.inv_temp));
 }
 
@@ -1074,29 +754,13 @@ template <typename T>
 cudaError_t launch_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
                           cudaStream_t stream) {
   const PolicyTerms q = *a.policy;
-  const bool ent = q.entropy_coef != 0.f;
-  const int64_t bytes = a.vocab * static_cast<int64_t>(sizeof(T)), sms = sm_count();
-  const auto slice = [&](int64_t ranks) { return ((bytes / 16 + ranks - 1) / ranks + 7) / 8 * 128; };
-  if (bytes < kRingLeast || slice(kMaxCluster) > kRingMost) {
-    return launch_rows(ent ? token_policy_kernel<T, true> : token_policy_kernel<T, false>,
-                       row_launch(a.rows, a.vocab, sizeof(T), true, 1), stream, a, q, grad, scale, scale_device, mean,
-                       base_of(a.inv_temp));
-  }
-  RowLaunch l;
-  l.threads = kRingThreads + 64;
-  l.ranks = 1;
-  while (l.ranks < kMaxCluster &&
-         (slice(l.ranks) > kRingSlice || (a.rows * l.ranks * 2 <= 2 * sms && slice(l.ranks) >= 16 * kRingThreads * 2))) {
-    l.ranks *= 2;
-  }
-  const int stage = static_cast<int>(slice(l.ranks));
-  l.smem = stage * kStages;
-  const auto kern = ent ? token_policy_ring_kernel<T, true> : token_policy_ring_kernel<T, false>;
+  const auto kern = q.entropy_coef != 0.f ? token_policy_kernel<T, true> : token_policy_kernel<T, false>;
+  RowLaunch l = row_launch(a.rows, a.vocab, sizeof(T), true);
   int resident = 0;
   const cudaError_t e = resident_clusters(kern, l, &resident);
   if (e != cudaSuccess) return e;
   l.clusters = std::min<int64_t>(a.rows, resident);
-  return launch_rows(kern, l, stream, a, q, grad, scale, scale_device, mean, base_of(a.inv_temp), stage);
+  return launch_rows(kern, l, stream, a, q, grad, scale, scale_device, mean, base_of(a.inv_temp));
 }
 
 // ---- gradient of the logits from the row statistics -----------------------------------------------------------------------
@@ -1196,25 +860,35 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {  // re
   }
 }
 
-constexpr int kFinishThreads = 512;
+constexpr int kFinishThreads = 1024;
 __global__ void __launch_bounds__(kFinishThreads) policy_finish_kernel(const PolicyFinishArgs a) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
   __shared__ double s_sum[kFinishThreads / 32 * 5];
   double x[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
-  for (int64_t r = threadIdx.x; r < a.rows; r += kFinishThreads) {
-    const float4 t = a.terms[r];
-    float w;
-    row_token(a.idx, r, a.vocab, w);
-    x[0] += t.x, x[1] += t.y, x[2] += t.z, x[3] += t.w, x[4] += w;
+  constexpr int kRows = 4;  // in flight per thread
+  for (int64_t r0 = threadIdx.x; r0 < a.rows; r0 += kRows * kFinishThreads) {
+    float4 t[kRows];
+    float w[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const int64_t r = r0 + j * kFinishThreads;
+      t[j] = make_float4(0.f, 0.f, 0.f, 0.f), w[j] = 0.f;
+      if (r < a.rows) {
+        t[j] = a.terms[r];
+        row_token(a.idx, r, a.vocab, w[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) x[0] += t[j].x, x[1] += t[j].y, x[2] += t[j].z, x[3] += t[j].w, x[4] += w[j];
   }
   block_sum(x, s_sum);
   if (threadIdx.x == 0) {
     const double inv = x[4] != 0.0 ? 1.0 / x[4] : 0.0;  // no row counts: loss and gradients are zero
     const double f = a.mean ? inv : 1.0;
-    a.out[0] = static_cast<float>(f * (x[0] + a.kl_coef * x[1] - a.entropy_coef * x[2]));
-    for (int n = 0; n < 4; ++n) a.out[1 + n] = static_cast<float>(inv * x[n]);
-    a.out[5] = static_cast<float>(f);
+    a.loss[0] = static_cast<float>(f * (x[0] + a.kl_coef * x[1] - a.entropy_coef * x[2]));
+    for (int n = 0; n < 4; ++n) a.out[n] = static_cast<float>(inv * x[n]);
+    a.out[4] = static_cast<float>(f);
   }
 }
 
@@ -1226,72 +900,101 @@ __device__ __forceinline__ int64_t seq_start(const PreferenceArgs& a, int64_t s)
 }
 
 // -log sigmoid(x)
-__device__ __forceinline__ double softplus_neg(double x) { return log1p(exp(-fabs(x))) + fmax(-x, 0.0); }
+__device__ __forceinline__ float softplus_neg(float x) { return log1pf(expf(-fabsf(x))) + fmaxf(-x, 0.f); }
 
 constexpr int kPairThreads = 1024;
-// One block: a warp per sequence sums its tokens' log-probabilities in 64 bits, then the pairs' losses, then every row's
-// coefficient. Tens of thousands of rows are a few hundred kilobytes, so one block's time stays far below the logits'.
+// One block, split into teams of threads: a team sums the log-probabilities of a pair's two sequences (in 64 bits, in a
+// fixed order), its first thread works out the pair's loss, and the team writes the rows' coefficients. Tens of thousands
+// of rows are a few hundred kilobytes, so one block's time stays far below the logits'.
 __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const PreferenceArgs a) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
-  __shared__ double s_sum[kPairThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kPairThreads / 32;
+  __shared__ double s_part[kPairThreads / 32][4];
+  __shared__ float s_coef[kPairThreads / 32][2];
+  __shared__ double s_loss[kPairThreads / 32];
   for (int64_t r = threadIdx.x; r < a.rows; r += kPairThreads) a.coef[r] = 0.f;
-  __syncthreads();
-  double loss[1] = {0.0};
   const int64_t pairs = a.seqs / 2;
-  for (int64_t p = warp; p < pairs; p += warps) {
-    double sum[2], count[2], lp[2];
-    for (int c = 0; c < 2; ++c) {
-      const int64_t r0 = seq_start(a, 2 * p + c), r1 = seq_start(a, 2 * p + c + 1);
-      sum[c] = 0.0, count[c] = 0.0;
-      for (int64_t r = r0 + lane; r < r1; r += 32) {
-        float w;
-        if (row_token(a.idx, r, a.vocab, w) < 0) continue;
-        sum[c] += static_cast<double>(w) * a.logp[r];
-        count[c] += w;
+  int teams = 1;
+  while (teams < kPairThreads / 32 && teams < pairs) teams *= 2;
+  const int size = kPairThreads / teams, team = threadIdx.x / size, t = threadIdx.x % size;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = size / 32;
+  double loss = 0.0;
+  for (int64_t base = 0; base < pairs; base += teams) {
+    const int64_t p = base + team;
+    int64_t at[3] = {0, 0, 0};
+    double x[4] = {0.0, 0.0, 0.0, 0.0};  // sums and weights of the two sequences
+    if (p < pairs) {
+      for (int c = 0; c < 3; ++c) at[c] = seq_start(a, 2 * p + c);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        for (int64_t r = at[c] + t; r < at[c + 1]; r += size) {
+          float w;
+          const float logp = a.logp[r];
+          if (row_token(a.idx, r, a.vocab, w) < 0) continue;
+          x[c] += static_cast<double>(w) * logp;
+          x[2 + c] += w;
+        }
       }
-      for (int o = 16; o >= 1; o >>= 1) {
-        sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], o);
-        count[c] += __shfl_xor_sync(0xffffffffu, count[c], o);
+    }
+    for (int n = 0; n < 4; ++n) {
+      for (int o = 16; o >= 1; o >>= 1) x[n] += __shfl_xor_sync(0xffffffffu, x[n], o);
+    }
+    __syncthreads();  // the rows are cleared, the last pairs' partial sums and coefficients have been read
+    if (lane == 0) {
+      for (int n = 0; n < 4; ++n) s_part[warp][n] = x[n];
+    }
+    __syncthreads();
+    if (t == 0 && p < pairs) {
+      for (int n = 0; n < 4; ++n) {
+        x[n] = 0.0;
+        for (int i = 0; i < warps; ++i) x[n] += s_part[warp + i][n];
       }
-      lp[c] = !a.average ? sum[c] : count[c] != 0.0 ? sum[c] / count[c] : 0.0;
-    }
-    double rew[2];
-    for (int c = 0; c < 2; ++c) rew[c] = a.beta * (lp[c] - (a.ref ? static_cast<double>(a.ref[2 * p + c]) : 0.0));
-    const double h = rew[0] - rew[1];
-    double l, dh;  // loss of the pair and its derivative by h
-    if (a.kind == kPrefSigmoid) {
-      l = (1.0 - a.smoothing) * softplus_neg(h) + a.smoothing * softplus_neg(-h);
-      dh = a.smoothing / (1.0 + exp(-h)) - (1.0 - a.smoothing) / (1.0 + exp(h));
-    } else if (a.kind == kPrefHinge) {
-      l = fmax(1.0 - h, 0.0);
-      l = isnan(h) ? h : l;
-      dh = h < 1.0 ? -1.0 : 0.0;
-    } else {  // squared distance of the log-ratio difference h / beta from 1 / (2 beta)
-      const double d = h / a.beta - 0.5 / a.beta;
-      l = d * d;
-      dh = 2.0 * d / a.beta;
-    }
-    if (lane == 0) loss[0] += l;
-    const double g = dh * a.beta / static_cast<double>(pairs);
-    for (int c = 0; c < 2; ++c) {
-      if (lane == 0) {
+      double lp[2], rew[2];
+      for (int c = 0; c < 2; ++c) {
+        lp[c] = !a.average ? x[c] : x[2 + c] != 0.0 ? x[c] / x[2 + c] : 0.0;
+        rew[c] = a.beta * (lp[c] - (a.ref ? static_cast<double>(a.ref[2 * p + c]) : 0.0));
         a.seq_logp[2 * p + c] = static_cast<float>(lp[c]);
         a.rewards[2 * p + c] = static_cast<float>(rew[c]);
       }
-      double gc = c == 0 ? g : -g;
-      if (a.average) gc = count[c] != 0.0 ? gc / count[c] : 0.0;
-      const int64_t r0 = seq_start(a, 2 * p + c), r1 = seq_start(a, 2 * p + c + 1);
-      for (int64_t r = r0 + lane; r < r1; r += 32) {
-        float w;
-        row_token(a.idx, r, a.vocab, w);
-        a.coef[r] = static_cast<float>(gc * w);
+      const float h = static_cast<float>(rew[0] - rew[1]);
+      float l, dh;  // loss of the pair and its derivative by h
+      if (a.kind == kPrefSigmoid) {
+        l = (1.f - a.smoothing) * softplus_neg(h) + a.smoothing * softplus_neg(-h);
+        dh = a.smoothing / (1.f + expf(-h)) - (1.f - a.smoothing) / (1.f + expf(h));
+      } else if (a.kind == kPrefHinge) {
+        l = isnan(h) ? h : fmaxf(1.f - h, 0.f);
+        dh = h < 1.f ? -1.f : 0.f;
+      } else {  // squared distance of the log-ratio difference h / beta from 1 / (2 beta)
+        const double d = (rew[0] - rew[1] - 0.5) / a.beta;
+        l = static_cast<float>(d * d);
+        dh = static_cast<float>(2.0 * d / a.beta);
+      }
+      loss += l;
+      const double g = static_cast<double>(dh) * a.beta / static_cast<double>(pairs);
+      for (int c = 0; c < 2; ++c) {
+        const double gc = c == 0 ? g : -g;
+        s_coef[team][c] = static_cast<float>(!a.average ? gc : x[2 + c] != 0.0 ? gc / x[2 + c] : 0.0);
+      }
+    }
+    __syncthreads();
+    if (p < pairs) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        for (int64_t r = at[c] + t; r < at[c + 1]; r += size) {
+          float w;
+          row_token(a.idx, r, a.vocab, w);
+          a.coef[r] = s_coef[team][c] * w;
+        }
       }
     }
   }
-  block_sum(loss, s_sum);
-  if (threadIdx.x == 0) a.loss[0] = pairs ? static_cast<float>(loss[0] / static_cast<double>(pairs)) : 0.f;
+  if (t == 0) s_loss[team] = loss;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    loss = 0.0;
+    for (int i = 0; i < teams; ++i) loss += s_loss[i];
+    a.loss[0] = pairs ? static_cast<float>(loss / static_cast<double>(pairs)) : 0.f;
+  }
 }
 
 }  // namespace

@@ -72,7 +72,7 @@ struct TokenGradArgs {
 };
 cudaError_t token_grad(const TokenGradArgs& a, cudaStream_t stream);
 
-// out[0..5] = loss, surrogate, kl, entropy, clip fraction, factor that the gradients carry (1 / sum of weights, or 1).
+// loss[0]; out[0..4] = surrogate, kl, entropy, clip fraction, factor that the gradients carry (1 / sum of weights, or 1).
 struct PolicyFinishArgs {
   int64_t rows;
   const float4* terms;
@@ -80,7 +80,7 @@ struct PolicyFinishArgs {
   int64_t vocab;
   float kl_coef, entropy_coef;
   int mean;
-  float* out;
+  float *loss, *out;
 };
 cudaError_t policy_finish(const PolicyFinishArgs& a, cudaStream_t stream);
 

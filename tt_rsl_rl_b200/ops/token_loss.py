@@ -188,26 +188,21 @@ def _policy_torch(logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind,
     return TokenPolicyLoss((loss * inv if mean else loss).float(), *stats, logp.detach())
 
 
-def _policy_result(out: torch.Tensor, logp: torch.Tensor, loss: torch.Tensor | None = None) -> TokenPolicyLoss:
-    parts = out.unbind()
-    return TokenPolicyLoss(parts[0] if loss is None else loss, *parts[1:5], logp)
-
-
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, old, adv, ref, mask, settings, temperature):
         lo, hi, kl_coef, kl_kind, entropy_coef, mean = settings
-        out, logp, entropy, stats, coef = ext().token_policy_loss(
+        loss, *means, factor, logp, entropy, stats, coef = ext().token_policy_loss(
             logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind, entropy_coef, temperature, mean, False, 1.0,
             None)
-        ctx.save_for_backward(logits, tokens, mask, stats, entropy if entropy_coef != 0.0 else None, coef, out[5])
+        ctx.save_for_backward(logits, tokens, mask, stats, entropy if entropy_coef != 0.0 else None, coef, factor)
         ctx.temperature = temperature
-        ctx.mark_non_differentiable(out, logp)
-        return out[0].clone(), out, logp
+        ctx.mark_non_differentiable(*means, logp)
+        return loss, *means, logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, _d_out, _d_logp):
+    def backward(ctx, d_loss, *_):
         _refuse_capture("token_policy_loss")
         logits, tokens, mask, stats, entropy, coef, factor = ctx.saved_tensors
         grad = ext().token_loss_backward(logits, tokens, mask, ctx.temperature, stats, entropy, coef, factor, d_loss)
@@ -234,11 +229,11 @@ def token_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torc
         return _policy_torch(logits, tokens, old_logp, advantages, ref_logp, mask, *settings, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_capture("token_policy_loss")
-        loss, out, logp = _PolicyLoss.apply(logits, tokens, old_logp, advantages, ref_logp, mask, settings, temperature)
-        return _policy_result(out, logp, loss)
-    out, logp, *_ = ext().token_policy_loss(logits, tokens, old_logp, advantages, ref_logp, mask, *settings[:5],
-                                            temperature, settings[5], False, 1.0, None)
-    return _policy_result(out, logp)
+        return TokenPolicyLoss(*_PolicyLoss.apply(logits, tokens, old_logp, advantages, ref_logp, mask, settings,
+                                                  temperature))
+    parts = ext().token_policy_loss(logits, tokens, old_logp, advantages, ref_logp, mask, *settings[:5], temperature,
+                                    settings[5], False, 1.0, None)
+    return TokenPolicyLoss(*parts[:5], parts[6])
 
 
 def _split_scale(grad_scale):
@@ -263,9 +258,9 @@ def token_policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logp:
                            mask=mask, clip_param=clip_param, clip_high=clip_high, kl_coef=kl_coef,
                            kl_estimator=kl_estimator, entropy_coef=entropy_coef, temperature=temperature,
                            reduction=reduction)
-    out, logp, grad = ext().token_policy_loss(logits.detach(), tokens, old_logp, advantages, ref_logp, mask,
-                                              *settings[:5], temperature, settings[5], True, scale, scale_device)
-    return _policy_result(out, logp), grad
+    parts = ext().token_policy_loss(logits, tokens, old_logp, advantages, ref_logp, mask, *settings[:5], temperature,
+                                    settings[5], True, scale, scale_device)
+    return TokenPolicyLoss(*parts[:5], parts[6]), parts[7]
 
 
 def _grad_torch(loss_fn, logits, grad_scale, *args, **kwargs):
@@ -388,6 +383,6 @@ def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: 
         return _grad_torch(preference_loss, logits, grad_scale, tokens, ref_logps, offsets=offsets, mask=mask, beta=beta,
                            label_smoothing=label_smoothing, loss_type=loss_type, average=average,
                            temperature=temperature)
-    loss, seq, rewards, logp, grad = ext().preference_loss(logits.detach(), tokens, ref_logps, offsets, mask, *settings,
+    loss, seq, rewards, logp, grad = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings,
                                                            temperature, True, scale, scale_device)
     return PreferenceLoss(loss, rewards[0::2], rewards[1::2], seq, logp), grad
