@@ -201,7 +201,9 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   q.clip_lo = static_cast<float>(clip_lo), q.clip_hi = static_cast<float>(clip_hi);
   q.kl_coef = static_cast<float>(kl_coef), q.entropy_coef = static_cast<float>(entropy_coef);
   q.kl_kind = static_cast<int>(kl_kind);
-  Tensor loss = torch::empty({}, l.f32()), out = torch::empty({5}, l.f32()), logp = torch::empty(l.lead(), l.f32());
+  // the loss is a tensor of its own where autograd takes it, else (one allocation less) a view like the means
+  Tensor out = torch::empty({6}, l.f32()), logp = torch::empty(l.lead(), l.f32()), loss;
+  if (!want_grad) loss = torch::empty({}, l.f32());
   Tensor terms = torch::empty({l.rows, 4}, l.f32()), entropy, ml, coef, grad;
   if (want_grad) grad = l.gradient();
   const bool one_pass = want_grad && l.same_phase(grad);
@@ -224,10 +226,11 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   }
   rlb::PolicyFinishArgs f{};
   f.rows = l.rows, f.terms = a.terms, f.idx = ix.idx, f.vocab = l.vocab, f.kl_coef = q.kl_coef;
-  f.entropy_coef = q.entropy_coef, f.mean = mean, f.loss = loss.data_ptr<float>(), f.out = out.data_ptr<float>();
+  f.entropy_coef = q.entropy_coef, f.mean = mean;
+  f.loss = want_grad ? out.data_ptr<float>() : loss.data_ptr<float>(), f.out = out.data_ptr<float>() + 1;
   ok(rlb::policy_finish(f, stream), "token_policy_loss");
   std::vector<Tensor> result = out.unbind();
-  result.insert(result.begin(), loss);
+  if (!want_grad) result[0] = loss;
   result.push_back(logp);
   if (!want_grad) {
     result.insert(result.end(), {entropy, ml, coef});
@@ -242,7 +245,7 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
     if (q.entropy_coef != 0.f) g.b = coef.data_ptr<float>() + 1, g.b_stride = 2;
     g.weighted = 1;
     g.scale = static_cast<float>(grad_scale), g.scale_a = scale_device;
-    g.scale_b = out.data_ptr<float>() + 4;
+    g.scale_b = out.data_ptr<float>() + 5;
     ok(rlb::token_grad(g, stream), "token_policy_loss");
   }
   result.push_back(grad);
@@ -277,7 +280,7 @@ Tensor token_loss_backward(const Tensor& logits, const Tensor& tokens, const Opt
 }
 
 // ---- preference loss ----------------------------------------------------------------------------------------------------
-// Returns [loss, seq_logp, rewards, logp, grad] with want_grad, [loss, seq_logp, rewards, logp, ml, coef] without.
+// Returns loss, chosen rewards, rejected rewards, seq_logp, logp, then [grad] with want_grad, [ml, coef] without.
 std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, const OptT& ref, const OptT& offsets,
                                     const OptT& mask, double beta, double smoothing, int64_t kind, bool average,
                                     double temperature, bool want_grad, double grad_scale,
@@ -311,9 +314,12 @@ std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, 
     r = ref->contiguous();
     p.ref = r.data_ptr<float>();
   }
-  Tensor loss = torch::empty({}, l.f32()), seq = torch::empty({p.seqs}, l.f32()), rew = torch::empty({p.seqs}, l.f32());
+  Tensor loss = torch::empty({}, l.f32()), seq = torch::empty({p.seqs}, l.f32()), rew = torch::empty({2, p.seqs / 2}, l.f32());
   Tensor logp = torch::empty(l.lead(), l.f32()), ml = torch::empty({l.rows, 2}, l.f32());
   Tensor coef = torch::empty({l.rows}, l.f32());
+  std::vector<Tensor> result = rew.unbind();
+  result.insert(result.begin(), loss);
+  result.insert(result.end(), {seq, logp});
   rlb::TokenStatsArgs a{};
   a.dtype = l.dtype, a.rows = l.rows, a.vocab = l.vocab, a.z = l.z, a.idx = ix.idx, a.inv_temp = inverse(temperature);
   a.logp = logp.data_ptr<float>();
@@ -325,7 +331,10 @@ std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, 
   p.loss = loss.data_ptr<float>(), p.seq_logp = seq.data_ptr<float>(), p.rewards = rew.data_ptr<float>();
   p.coef = coef.data_ptr<float>();
   ok(rlb::preference_pairs(p, stream), "preference_loss");
-  if (!want_grad) return {loss, seq, rew, logp, ml, coef};
+  if (!want_grad) {
+    result.insert(result.end(), {ml, coef});
+    return result;
+  }
   Tensor grad = l.gradient();
   rlb::TokenGradArgs g{};
   g.dtype = l.dtype, g.rows = l.rows, g.vocab = l.vocab, g.z = l.z, g.idx = ix.idx, g.inv_temp = a.inv_temp;
@@ -335,7 +344,8 @@ std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, 
   g.weighted = 1;
   g.scale = static_cast<float>(grad_scale), g.scale_a = scale_ptr(l, grad_scale_device);
   ok(rlb::token_grad(g, stream), "preference_loss");
-  return {loss, seq, rew, logp, grad};
+  result.push_back(grad);
+  return result;
 }
 
 // ---- AdamW ------------------------------------------------------------------------------------------------------------

@@ -19,7 +19,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr double kLog2e = 1.4426950408889634;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f, kLn2Lack = -1.90465429995776e-9f;  // ln 2 as a sum
 constexpr float kFar = -1e30f;  // exponent of a column of probability zero: its product with that zero stays a number
 
 __device__ __forceinline__ float ex2(float x) {
@@ -299,10 +299,10 @@ __device__ __forceinline__ void soft_warp_reduce(Soft& a, const Base& k) {
   }
 }
 
-// What a row's sums say: ln sum_j e^((z_j - m) / T) = lns + fix, where lns is of the sums as they are and fix (about 1e-6)
-// what the rounding of c and of hi has shifted. Kept apart, and all in fp32: fp64 runs at a thirtieth of its rate.
+// What a row's sums say: ln sum_j e^((z_j - m) / T) = lns + rest, where lns is a multiple of ln 2 and the rest below one, so
+// that a log-probability is rounded once. The rest has what the rounding of c and of hi has shifted (about 1e-6).
 struct RowSoft {
-  float m, lns, fix;
+  float m, lns, rest;
   float mean;  // of z - m under p
   float entropy;
 };
@@ -310,23 +310,31 @@ __device__ __forceinline__ RowSoft row_soft(const Soft& a, const Base& k) {
   RowSoft r;
   r.m = a.m;
   const float off = a.m > kLow ? fmaf(a.m, k.hi, shift_of(a.m, k)) : 0.f;  // exact
-  r.lns = logf(a.s);
+  const uint32_t bits = __float_as_uint(a.s);
+  const bool normal = a.s > 1e-30f && a.s < 1e30f;
+  const float e = normal ? static_cast<float>(static_cast<int>(bits >> 23) - 127) : 0.f;
+  const float f = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : a.s;
+  r.lns = e * kLn2;
   const float td = a.t / a.s;
   r.mean = (td - off) / k.hi;
-  r.fix = kLn2 * fmaf(k.lo, r.mean, -off);
-  r.entropy = r.lns - td * kLn2;
+  const float rest = logf(f) + (fmaf(e, kLn2, -r.lns) + e * kLn2Lack);  // of the sums as they are
+  r.rest = rest + kLn2 * fmaf(k.lo, r.mean, -off);
+  r.entropy = r.lns + (rest - td * kLn2);
   return r;
 }
 __device__ __forceinline__ float row_logp(const RowSoft& r, float z, const Base& k) {
   const float d = z - r.m;
-  return (isinf(d) ? d : fmaf(d, k.inv, d * k.inv_lack)) - r.lns - r.fix;
+  if (isinf(d)) return d - r.lns - r.rest;
+  const float x = fmaf(d, k.inv, d * k.inv_lack), y = x - r.lns;
+  const float back = y + r.lns;  // the rounding of y by the two-sum
+  return y + (((x - back) + (back - y - r.lns)) - r.rest);
 }
 // What a gradient needs of a row: p_j = f 2^(z_j hi + c), f the rounding of c to a float; f < 0 marks a row of lowest
 // values: p_j = 2^((z_j - c) hi + 1 + f).
 __device__ __forceinline__ float2 row_shift(const RowSoft& r, const Base& k) {
   constexpr float kE = 1.44269504f, kELack = 1.92596299e-8f;  // log2(e) as a sum
-  const float l = r.lns * kE, l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.fix * kE;
-  if (!(r.m > kLow)) return make_float2(r.m, -1.f - l);
+  const float l = r.lns * kE, l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.rest * kE;
+  if (!(r.m > kLow)) return make_float2(r.m, -1.f - (l + l_lack));
   const float p = r.m * k.hi, p_lack = fmaf(r.m, k.hi, -p);
   const float c = -(p + l), t = -c - p;  // c's own rounding by the two-sum
   const float lack = (p - (-c - t)) + (l - t) + p_lack + l_lack;
@@ -840,8 +848,9 @@ cudaError_t launch_grad(const TokenGradArgs& a, cudaStream_t stream) {
 }
 
 // ---- sums over rows, sequences and pairs -----------------------------------------------------------------------------------
+// Sums of a block in fixed order, in every thread. smem: N numbers per warp.
 template <int N>
-__device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {  // result in every thread; fixed order
+__device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -853,11 +862,14 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {  // re
     for (int n = 0; n < N; ++n) smem[warp * N + n] = x[n];
   }
   __syncthreads();
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    x[n] = 0.0;
-    for (int i = 0; i < warps; ++i) x[n] += smem[i * N + n];
+  if (threadIdx.x < N) {  // fp64 adds are slow: one thread for each sum
+    double y = smem[threadIdx.x];
+    for (int i = 1; i < warps; ++i) y += smem[i * N + threadIdx.x];
+    smem[threadIdx.x] = y;
   }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = smem[n];
 }
 
 constexpr int kFinishThreads = 1024;
@@ -927,12 +939,24 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
       for (int c = 0; c < 3; ++c) at[c] = seq_start(a, 2 * p + c);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        for (int64_t r = at[c] + t; r < at[c + 1]; r += size) {
-          float w;
-          const float logp = a.logp[r];
-          if (row_token(a.idx, r, a.vocab, w) < 0) continue;
-          x[c] += static_cast<double>(w) * logp;
-          x[2 + c] += w;
+        constexpr int kRows = 4;  // in flight per thread
+        for (int64_t r0 = at[c] + t; r0 < at[c + 1]; r0 += kRows * size) {
+          float logp[kRows], w[kRows];
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            const int64_t r = r0 + j * size;
+            logp[j] = w[j] = 0.f;
+            if (r < at[c + 1]) {
+              logp[j] = a.logp[r];
+              row_token(a.idx, r, a.vocab, w[j]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kRows; ++j) {
+            if (w[j] == 0.f) continue;
+            x[c] += static_cast<double>(w[j]) * logp[j];
+            x[2 + c] += w[j];
+          }
         }
       }
     }
@@ -954,7 +978,7 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
         lp[c] = !a.average ? x[c] : x[2 + c] != 0.0 ? x[c] / x[2 + c] : 0.0;
         rew[c] = a.beta * (lp[c] - (a.ref ? static_cast<double>(a.ref[2 * p + c]) : 0.0));
         a.seq_logp[2 * p + c] = static_cast<float>(lp[c]);
-        a.rewards[2 * p + c] = static_cast<float>(rew[c]);
+        a.rewards[c * pairs + p] = static_cast<float>(rew[c]);
       }
       const float h = static_cast<float>(rew[0] - rew[1]);
       float l, dh;  // loss of the pair and its derivative by h
@@ -980,10 +1004,12 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
     if (p < pairs) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        const float coef = s_coef[team][c];
+#pragma unroll 4
         for (int64_t r = at[c] + t; r < at[c + 1]; r += size) {
           float w;
           row_token(a.idx, r, a.vocab, w);
-          a.coef[r] = s_coef[team][c] * w;
+          a.coef[r] = coef * w;
         }
       }
     }

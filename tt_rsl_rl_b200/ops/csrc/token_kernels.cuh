@@ -96,7 +96,7 @@ struct PreferenceArgs {
   int kind, average;
   float* loss;        // [1]
   float* seq_logp;    // [seqs]
-  float* rewards;     // [seqs]
+  float* rewards;     // [2, seqs / 2]: of the chosen, of the rejected sequences
   float* coef;        // [rows] dL/dlogp; zero outside the sequences
 };
 cudaError_t preference_pairs(const PreferenceArgs& a, cudaStream_t stream);

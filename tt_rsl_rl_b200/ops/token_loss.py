@@ -153,11 +153,13 @@ def _policy_settings(ref_logp, clip_param, clip_high, kl_coef, kl_estimator, ent
         raise ValueError(f"kl_estimator must be one of {list(KL_ESTIMATORS)}, got {kl_estimator!r}")
     if reduction not in ("mean", "sum"):
         raise ValueError(f"reduction must be 'mean' or 'sum', got {reduction!r}")
-    clip_param = _finite("clip_param", clip_param)
-    clip_high = clip_param if clip_high is None else _finite("clip_high", clip_high)
+    if clip_high is None:
+        clip_high = clip_param
+    if not math.isfinite(clip_param + clip_high + kl_coef + entropy_coef):
+        raise ValueError(f"clip_param, clip_high, kl_coef and entropy_coef must be finite, got {clip_param}, {clip_high}, "
+                         f"{kl_coef} and {entropy_coef}")
     if clip_param < 0.0 or clip_high < 0.0:
         raise ValueError(f"clip_param and clip_high must not be negative, got {clip_param} and {clip_high}")
-    kl_coef, entropy_coef = _finite("kl_coef", kl_coef), _finite("entropy_coef", entropy_coef)
     if kl_coef != 0.0 and ref_logp is None:
         raise ValueError("kl_coef needs ref_logp")
     return 1.0 - clip_param, 1.0 + clip_high, kl_coef, KL_ESTIMATORS[kl_estimator], entropy_coef, reduction == "mean"
@@ -328,12 +330,12 @@ def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind,
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, ref, offsets, mask, settings, temperature):
-        loss, seq, rewards, logp, stats, coef = ext().preference_loss(logits, tokens, ref, offsets, mask, *settings,
-                                                                      temperature, False, 1.0, None)
+        loss, *parts, stats, coef = ext().preference_loss(logits, tokens, ref, offsets, mask, *settings, temperature,
+                                                          False, 1.0, None)
         ctx.save_for_backward(logits, tokens, mask, stats, coef)
         ctx.temperature = temperature
-        ctx.mark_non_differentiable(seq, rewards, logp)
-        return loss, seq, rewards, logp
+        ctx.mark_non_differentiable(*parts)
+        return loss, *parts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -364,11 +366,9 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: torch
         return _preference_torch(logits, tokens, ref_logps, offsets, mask, *settings, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_capture("preference_loss")
-        loss, seq, rewards, logp = _PreferenceLoss.apply(logits, tokens, ref_logps, offsets, mask, settings, temperature)
-    else:
-        loss, seq, rewards, logp, *_ = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings,
-                                                             temperature, False, 1.0, None)
-    return PreferenceLoss(loss, rewards[0::2], rewards[1::2], seq, logp)
+        return PreferenceLoss(*_PreferenceLoss.apply(logits, tokens, ref_logps, offsets, mask, settings, temperature))
+    parts = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings, temperature, False, 1.0, None)
+    return PreferenceLoss(*parts[:5])
 
 
 def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
@@ -383,6 +383,6 @@ def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: 
         return _grad_torch(preference_loss, logits, grad_scale, tokens, ref_logps, offsets=offsets, mask=mask, beta=beta,
                            label_smoothing=label_smoothing, loss_type=loss_type, average=average,
                            temperature=temperature)
-    loss, seq, rewards, logp, grad = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings,
-                                                           temperature, True, scale, scale_device)
-    return PreferenceLoss(loss, rewards[0::2], rewards[1::2], seq, logp), grad
+    *parts, grad = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings, temperature, True, scale,
+                                         scale_device)
+    return PreferenceLoss(*parts), grad
