@@ -48,6 +48,9 @@ struct AdamFactors {
 
 struct AdamConsts {
   double max_norm;
+  // -0: the assembler fuses mul.rn.f32x2 and add.rn.f32x2 into one rounding (unlike their single forms), but not a product
+  // that is a fused multiply-add with an addend it does not know
+  float none;
   float beta1, beta1c, beta2, beta2c, eps;
   int maximize;
   uint32_t first_stream;
@@ -191,23 +194,26 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 // 20 to 26, and four of them packed at the end.
 constexpr float kUp = 1.329227995784916e36f, kDown = 7.52316384526264e-37f;  // 2^120, 2^-120
 constexpr uint32_t kCode = 1u << 20;
-__device__ __forceinline__ float code_value(uint32_t bits) { return __uint_as_float(bits) * kUp; }
-// (rnd16 + 1 / 2) / 2^16 by its bits
-__device__ __forceinline__ float uniform(uint32_t rnd16) {
-  return __uint_as_float(0x3f800040u | rnd16 << 7) - 1.f;
-}
 // The code below or above y (0 <= y <= 448, or half a unit more by the scale's rounding): above with probability
 // (y - below) / (above - below), which is what the 20 bits under the code say. Rounding the scaled y up leaves a fraction
 // that is not zero above every fraction below it.
 __device__ __forceinline__ uint32_t linear_code(float y, uint32_t rnd16) {
   return __float_as_uint(__fmul_ru(y, kDown)) + (0xffff7u - 16u * rnd16);
 }
-// The same with probability (y^2 - below^2) / (above^2 - below^2).
-__device__ __forceinline__ uint32_t square_code(float y, uint32_t rnd16) {
-  const uint32_t below = __float_as_uint(__fmul_rz(y, kDown)) & 0xfff00000u;
-  const float lo = code_value(below), hi = code_value(below + kCode);
-  const bool up = __fmul_rn(__fmul_rn(hi - lo, hi + lo), uniform(rnd16)) < __fmul_rn(y - lo, y + lo);
-  return up ? below + kCode : below;
+// The same with probability (y^2 - below^2) / (above^2 - below^2), for two numbers.
+__device__ __forceinline__ void square_codes(const Pair& y, uint32_t rnd0, uint32_t rnd1, uint32_t (&code)[2]) {
+  float x[2], a[2], b[2];
+  y.split(x[0], x[1]);
+  const uint32_t c0 = __float_as_uint(__fmul_rz(x[0], kDown)) & 0xfff00000u;
+  const uint32_t c1 = __float_as_uint(__fmul_rz(x[1], kDown)) & 0xfff00000u;
+  const Pair up(kUp, kUp), minus(-1.f, -1.f);
+  const Pair lo = mul2(Pair(__uint_as_float(c0), __uint_as_float(c1)), up);
+  const Pair hi = mul2(Pair(__uint_as_float(c0 + kCode), __uint_as_float(c1 + kCode)), up);
+  const Pair u = add2(Pair(__uint_as_float(0x3f800040u | rnd0 << 7), __uint_as_float(0x3f800040u | rnd1 << 7)), minus);
+  mul2(mul2(fma2(lo, minus, hi), add2(hi, lo)), u).split(a[0], a[1]);
+  mul2(fma2(lo, minus, y), add2(y, lo)).split(b[0], b[1]);
+  code[0] = a[0] < b[0] ? c0 + kCode : c0;
+  code[1] = a[1] < b[1] ? c1 + kCode : c1;
 }
 // Bytes 3 of four words.
 __device__ __forceinline__ uint32_t pack_top(const uint32_t (&x)[4]) {
@@ -224,6 +230,34 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+// ---- correctly rounded roots and quotients, two at a time -----------------------------------------------------------------
+// P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor" (1990): Newton steps from an
+// approximation, then one step with the exact remainder. Right for 0 <= v < 1e30 and |a| < 1e30, 1e-20 <= d < 1e30 (below
+// about 1e-30 a result may be the neighbour of the rounded one); the functions of CUDA check for more and take one number.
+__device__ __forceinline__ Pair neg2(const Pair& a) { return mul2(a, Pair(-1.f, -1.f)); }
+
+__device__ __forceinline__ void sqrt2(const float (&v)[2], float (&r)[2]) {
+  float y[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) asm("rsqrt.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(fmaxf(v[i], __int_as_float(1))));  // zero stays zero below
+  const Pair x(v[0], v[1]), y2(y[0], y[1]), half(0.5f, 0.5f);
+  Pair g = mul2(x, y2), h = mul2(y2, half);
+  const Pair e = fma2(neg2(h), g, half);
+  g = fma2(g, e, g), h = fma2(h, e, h);
+  fma2(fma2(neg2(g), g, x), h, g).split(r[0], r[1]);
+}
+__device__ __forceinline__ Pair div2(const Pair& a, const Pair& d) {
+  float x[2], y[2];
+  d.split(x[0], x[1]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y[i]) : "f"(x[i]));
+  const Pair nd = neg2(d);
+  Pair y2(y[0], y[1]);
+  y2 = fma2(y2, fma2(nd, y2, Pair(1.f, 1.f)), y2);
+  const Pair q = mul2(a, y2);
+  return fma2(fma2(nd, q, a), y2, q);
 }
 
 // ---- the step ---------------------------------------------------------------------------------------------------------
@@ -338,11 +372,12 @@ struct Quad {
     if (kBits8) {
       unpack_codes(mc, m);
       unpack_codes(vc, v);
+      const Pair ms(m_scale, m_scale), vs(v_scale, v_scale);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        m[e] = __fmul_rn(m[e], m_scale);
-        const float r = __fmul_rn(v[e], v_scale);
-        v[e] = __fmul_rn(r, r);
+      for (int e = 0; e < 4; e += 2) {
+        mul2(Pair(m[e], m[e + 1]), ms).split(m[e], m[e + 1]);
+        const Pair r = mul2(Pair(v[e], v[e + 1]), vs);
+        mul2(r, r).split(v[e], v[e + 1]);
       }
     }
   }
@@ -368,14 +403,21 @@ struct Quad {
   // `v` holds the roots.
   __device__ __forceinline__ void encode_states(float m_inv, float v_inv, const Philox& rnd) {
     uint32_t x[4], y[4];
+    const Pair mi(m_inv, m_inv), vi(v_inv, v_inv);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      // the stored m is right on average
-      const uint32_t c = linear_code(__fmul_rn(fabsf(m[e]), m_inv), rnd.c[e] & 0xffffu);
-      x[e] = (c << 4 & 0x7f000000u) | (__float_as_uint(m[e]) & 0x80000000u);
-      // v, not its root, is right on average; never down to zero, which would leave m / eps as the next step
-      const uint32_t d = square_code(__fmul_rn(v[e], v_inv), rnd.c[e] >> 16);
-      y[e] = (v_inv > 0.f && v[e] > 0.f ? max(d, kCode) : d) << 4 & 0x7f000000u;
+    for (int e = 0; e < 4; e += 2) {
+      float z[2];
+      uint32_t d[2];
+      mul2(Pair(fabsf(m[e]), fabsf(m[e + 1])), mi).split(z[0], z[1]);
+      square_codes(mul2(Pair(v[e], v[e + 1]), vi), rnd.c[e] >> 16, rnd.c[e + 1] >> 16, d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // the stored m is right on average
+        x[e + i] = (linear_code(z[i], rnd.c[e + i] & 0xffffu) << 4 & 0x7f000000u) |
+                   (__float_as_uint(m[e + i]) & 0x80000000u);
+        // v, not its root, is right on average; never down to zero, which would leave m / eps as the next step
+        y[e + i] = (v_inv > 0.f && v[e + i] > 0.f ? max(d[i], kCode) : d[i]) << 4 & 0x7f000000u;
+      }
     }
     mc = pack_top(x);
     vc = pack_top(y);
@@ -402,6 +444,8 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_co
   }
   if (c.maximize) clip = -clip;
   const int lane = threadIdx.x & 31;
+  const Pair none(c.none, c.none), clip2(clip, clip), b1(c.beta1, c.beta1), b1c(c.beta1c, c.beta1c), b2(c.beta2, c.beta2),
+      b2c(c.beta2c, c.beta2c);
   walk_units(t, [&](int ti, uint32_t first, uint32_t units) {
     const Entry a = t.t[ti];
     const AdamFactors f = factors[ti];
@@ -417,27 +461,44 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_co
         else q[j].load_some(a, at + j * 128, left - j * 128 - lane * 4);
       }
       const float ms = kBits8 ? a.m_scale[u] : 0.f, vs = kBits8 ? a.v_scale[u] : 0.f;
-      float m_top = 0.f, r_top = 0.f;
+      float top[2] = {0.f, 0.f};  // of the moments: |m|, and for 8-bit states the root of v
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         q[j].decode(ms, vs);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float &p = q[j].p[e], &m = q[j].m[e], &v = q[j].v[e];
-          const float g = __fmul_rn(q[j].g[e], clip);
-          m = __fadd_rn(__fmul_rn(m, c.beta1), __fmul_rn(g, c.beta1c));
-          v = __fadd_rn(__fmul_rn(v, c.beta2), __fmul_rn(__fmul_rn(g, g), c.beta2c));
-          const float r = __fsqrt_rn(v);
-          const float x = __fdiv_rn(m, __fadd_rn(__fmul_rn(r, f.unbias), c.eps));
-          p = __fsub_rn(__fmul_rn(p, f.decay), __fmul_rn(f.step_size, x));
-          if (kBits8) {
-            v = r;
-            m_top = max_nan(m_top, fabsf(m));
-            r_top = max_nan(r_top, r);
+        for (int e = 0; e < 4; e += 2) {
+          float *m = q[j].m + e, *v = q[j].v + e;
+          const Pair g = mul2(Pair(q[j].g[e], q[j].g[e + 1]), clip2);
+          add2(fma2(Pair(m[0], m[1]), b1, none), fma2(g, b1c, none)).split(m[0], m[1]);
+          add2(fma2(Pair(v[0], v[1]), b2, none), fma2(mul2(g, g), b2c, none)).split(v[0], v[1]);
+          top[0] = max_nan(max_nan(top[0], fabsf(m[0])), fabsf(m[1]));
+          top[1] = max_nan(max_nan(top[1], v[0]), v[1]);
+        }
+      }
+      // the quick forms are for numbers: all lanes take the slow ones where one has to, and with a tiny eps
+      const bool quick = __all_sync(0xffffffffu, top[0] < 1e30f && top[1] < 1e30f) && c.eps >= 1e-20f;
+      const Pair unbias(f.unbias, f.unbias), eps(c.eps, c.eps), keep(f.decay, f.decay), rate(-f.step_size, -f.step_size);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float m[2] = {q[j].m[e], q[j].m[e + 1]}, v[2] = {q[j].v[e], q[j].v[e + 1]};
+          float r[2];
+          Pair x;
+          if (quick) {
+            sqrt2(v, r);
+            x = div2(Pair(m[0], m[1]), add2(fma2(Pair(r[0], r[1]), unbias, none), eps));
+          } else {
+            for (int i = 0; i < 2; ++i) r[i] = __fsqrt_rn(v[i]);
+            x = Pair(__fdiv_rn(m[0], __fadd_rn(__fmul_rn(r[0], f.unbias), c.eps)),
+                     __fdiv_rn(m[1], __fadd_rn(__fmul_rn(r[1], f.unbias), c.eps)));
           }
+          add2(fma2(Pair(q[j].p[e], q[j].p[e + 1]), keep, none), fma2(rate, x, none)).split(q[j].p[e], q[j].p[e + 1]);
+          if (kBits8) q[j].v[e] = r[0], q[j].v[e + 1] = r[1];
         }
       }
       if (kBits8) {
+        float m_top = top[0], r_top = __fsqrt_rn(top[1]);  // the root grows with its argument
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
           m_top = max_nan(m_top, __shfl_xor_sync(0xffffffffu, m_top, o));
@@ -541,7 +602,7 @@ cudaError_t step(const AdamLaunch& a, const AdamFactors* factors, Shared& sh, cu
   AdamConsts c{};
   c.beta1 = static_cast<float>(a.h.beta1), c.beta1c = static_cast<float>(1.0 - a.h.beta1);
   c.beta2 = static_cast<float>(a.h.beta2), c.beta2c = static_cast<float>(1.0 - a.h.beta2);
-  c.eps = static_cast<float>(a.h.eps), c.max_norm = sh.max_norm;
+  c.none = -0.f, c.eps = static_cast<float>(a.h.eps), c.max_norm = sh.max_norm;
   c.maximize = a.h.maximize, c.seed = a.h.seed, c.first_stream = a.first_stream;
   AdamTable<K> t;
   for (int first = 0; first < a.count; first += K) {

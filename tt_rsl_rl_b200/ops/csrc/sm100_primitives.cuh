@@ -262,6 +262,31 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16_f32(int M, int N, bool a_
          | (static_cast<uint32_t>(M >> 4) << 24);   // M / 16
 }
 
+// ---- packed fp32 ----------------------------------------------------------------------------------------------------
+// Two fp32 numbers in one instruction, each rounded as the single operation is: for kernels whose limit is the number of
+// instructions that they issue.
+struct Pair {
+  unsigned long long v;
+  Pair() = default;
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void split(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+  Pair y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return y;
+}
+__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
+  Pair y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+  return y;
+}
+__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
+  Pair y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
+  return y;
+}
+
 // ---- misc --------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void named_barrier_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

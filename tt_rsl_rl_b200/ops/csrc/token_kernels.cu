@@ -34,28 +34,6 @@ __device__ __forceinline__ float at_least_far(float d) {  // a NaN stays one
   return y;
 }
 
-// Two fp32 numbers in one instruction (sm_100): what these kernels issue, not what they compute, is their limit.
-struct Pair {
-  unsigned long long v;
-  Pair() = default;
-  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
-  __device__ __forceinline__ void split(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-};
-__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
-  Pair y;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return y;
-}
-__device__ __forceinline__ Pair add2(const Pair& a, const Pair& b) {
-  Pair y;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
-  return y;
-}
-__device__ __forceinline__ Pair mul2(const Pair& a, const Pair& b) {
-  Pair y;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y.v) : "l"(a.v), "l"(b.v));
-  return y;
-}
 __device__ __forceinline__ Pair ex2(const Pair& x) {
   float lo, hi;
   x.split(lo, hi);
