@@ -241,6 +241,9 @@ def refuse_plans(device):
         (ValueError, "need their scales", lambda x: x.pop("exp_avg_scales"), {"bits": 8}),
         (ValueError, "scales", lambda x: x["exp_avg_scales"].__setitem__(1, torch.zeros(1, device=device)), {"bits": 8}),
         (ValueError, "low_bits", lambda x: x.pop("low_bits"), {"dtype": torch.bfloat16}),
+        (ValueError, "share memory", lambda x: x.update(params=[x["params"][0]] * 2, m=[x["m"][0], x["m"][0].clone()],
+                                                        v=[x["v"][0], x["v"][0].clone()]), {}),
+        (ValueError, "share memory", lambda x: x["v"].__setitem__(1, x["m"][1]), {}),
     ]:
         with pytest.raises(error, match=text):
             plan(change, **kwargs)

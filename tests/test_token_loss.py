@@ -124,6 +124,8 @@ REFUSALS = [
     (TypeError, "advantages must be", dict(adv=lambda x: x.half())),
     (ValueError, "old_logp must have the shape", dict(old=lambda x: x.flatten())),
     (ValueError, "temperature", dict(temperature=0.0)),
+    (ValueError, "temperature", dict(temperature=float("nan"))),
+    (ValueError, "temperature", dict(temperature=1e-7)),
     (ValueError, "kl_estimator", dict(kl_estimator="k4")),
     (ValueError, "reduction", dict(reduction="none")),
     (ValueError, "negative", dict(clip_param=-0.1)),

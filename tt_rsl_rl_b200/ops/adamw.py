@@ -116,6 +116,11 @@ def _check_plan_cpu(params, m, v, steps, m_scales, v_scales, low) -> None:
                 raise TypeError(f"AdamWPlan: {name} {i} must be {want}, got {s.dtype}")
             if s.shape != p.shape or s.stride() != p.stride():
                 raise ValueError(f"AdamWPlan: {name} {i} must have the parameter's device, shape and strides")
+    apart = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                   for t in (*params, *m, *v, *m_scales, *v_scales, *low) if t.numel())
+    if any(b[0] < a[1] for a, b in zip(apart, apart[1:])):
+        raise ValueError("AdamWPlan: two tensors share memory")
+    for i, p in enumerate(params):
         for s in (m_scales[i], v_scales[i]) if m_scales else ():
             if s.dtype != torch.float32 or s.numel() != -(-p.numel() // BLOCK) or not s.is_contiguous():
                 raise ValueError(f"AdamWPlan: scales {i} must hold one float32 per {BLOCK} elements of the parameter")

@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -122,7 +123,7 @@ struct Index {
 };
 
 double inverse(double temperature) {
-  TORCH_CHECK_VALUE(std::isfinite(temperature) && temperature > 0.0, "temperature must be positive and finite, got ",
+  TORCH_CHECK_VALUE(temperature >= 1e-6 && temperature <= 1e6, "temperature must lie in [1e-6, 1e6], got ",
                     text(temperature));
   return 1.0 / temperature;
 }
@@ -204,7 +205,8 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   // the loss is a tensor of its own where autograd takes it, else (one allocation less) a view like the means
   Tensor out = torch::empty({6}, l.f32()), logp = torch::empty(l.lead(), l.f32()), loss;
   if (!want_grad) loss = torch::empty({}, l.f32());
-  Tensor terms = torch::empty({l.rows, 4}, l.f32()), entropy, ml, coef, grad;
+  // one row more than terms: the sum of the weights
+  Tensor terms = torch::empty({l.rows + 1, 4}, l.f32()), entropy, ml, coef, grad;
   if (want_grad) grad = l.gradient();
   const bool one_pass = want_grad && l.same_phase(grad);
   rlb::TokenStatsArgs a{};
@@ -214,7 +216,8 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
   a.terms = reinterpret_cast<float4*>(terms.data_ptr<float>());
   const float* scale_device = scale_ptr(l, grad_scale_device);
   if (one_pass) {
-    ok(rlb::token_policy(a, Logits::rows_of(grad), static_cast<float>(grad_scale), scale_device, mean, stream),
+    ok(rlb::token_policy(a, Logits::rows_of(grad), static_cast<float>(grad_scale), scale_device, mean,
+                         reinterpret_cast<double*>(terms.data_ptr<float>() + 4 * l.rows), stream),
        "token_policy_loss");
   } else {
     entropy = torch::empty(l.lead(), l.f32()), ml = torch::empty({l.rows, 2}, l.f32());
@@ -392,6 +395,7 @@ class AdamWPlan {
         check_scale(vs_[i], p, "exp_avg_sq_scales", i);
       }
     }
+    check_apart();
   }
 
   // The list of this step: every parameter that has a gradient. The list lives until the next call.
@@ -445,6 +449,20 @@ class AdamWPlan {
   c10::Device device() const { return steps_.device(); }
 
  private:
+  // All tensors are dense: each is one range of memory, and no two of them share any.
+  void check_apart() const {
+    std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    for (const auto* list : {&p_, &m_, &v_, &ms_, &vs_, &low_}) {
+      for (const Tensor& t : *list) {
+        const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+        if (t.numel()) ranges.emplace_back(at, at + t.numel() * t.element_size());
+      }
+    }
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i) {
+      TORCH_CHECK_VALUE(ranges[i].first >= ranges[i - 1].second, "AdamWPlan: two tensors share memory");
+    }
+  }
   static std::string number(size_t i) { return text(static_cast<int64_t>(i)); }
   static bool same_order(const Tensor& a, const Tensor& b) {
     for (int64_t d = 0; d < a.dim(); ++d) {

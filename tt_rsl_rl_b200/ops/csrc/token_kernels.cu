@@ -541,8 +541,29 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const Toke
 }
 
 // ---- policy loss and gradient in one pass -------------------------------------------------------------------------------
+// Sums of a block in fixed order, in every thread. smem: N numbers per warp.
 template <int N>
-__device__ __forceinline__ void block_sum(double (&x)[N], double* smem);
+__device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    for (int o = 16; o >= 1; o >>= 1) x[n] += __shfl_xor_sync(0xffffffffu, x[n], o);
+  }
+  __syncthreads();
+  if (lane == 0) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) smem[warp * N + n] = x[n];
+  }
+  __syncthreads();
+  if (threadIdx.x < N) {  // fp64 adds are slow: one thread for each sum
+    double y = smem[threadIdx.x];
+    for (int i = 1; i < warps; ++i) y += smem[i * N + threadIdx.x];
+    smem[threadIdx.x] = y;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = smem[n];
+}
 
 // A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
 // the rows in work fit L2 (row_ranks), so the logits come from memory once.
@@ -550,7 +571,7 @@ template <typename T, bool kEnt>
 __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                        const TokenRows grad, float scale,
                                                                        const float* scale_device, int mean,
-                                                                       const Base k) {
+                                                                       const double* weight_sum, const Base k) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
   constexpr int VN = Elem<T>::kPerVec;
@@ -561,14 +582,18 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int threads = blockDim.x;
   if (scale_device) scale *= *scale_device;
-  if (mean) {  // every CTA sums the weights for itself, in the same order
+  if (mean) {
     double total[1] = {0.0};
-    for (int64_t r = threadIdx.x; r < a.rows; r += threads) {
-      float w;
-      row_token(a.idx, r, a.vocab, w);
-      total[0] += w;
+    if (weight_sum != nullptr) {
+      total[0] = *weight_sum;
+    } else {  // few rows: every CTA sums the weights for itself, in the same order
+      for (int64_t r = threadIdx.x; r < a.rows; r += threads) {
+        float w;
+        row_token(a.idx, r, a.vocab, w);
+        total[0] += w;
+      }
+      block_sum(total, s_sum);
     }
-    block_sum(total, s_sum);
     scale *= total[0] != 0.0 ? static_cast<float>(1.0 / total[0]) : 0.f;
   }
   const float factor = scale * k.inv;
@@ -736,17 +761,43 @@ cudaError_t launch_stats(const TokenStatsArgs& a, cudaStream_t stream) {
                      a.policy != nullptr, base_of(a.inv_temp));
 }
 
+constexpr int kFinishThreads = 1024;
+__global__ void __launch_bounds__(kFinishThreads) policy_weights_kernel(const TokenIndex idx, int64_t rows, int64_t vocab,
+                                                                        double* out) {
+  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
+  griddep_launch_dependents();
+  __shared__ double s_sum[kFinishThreads / 32];
+  double x[1] = {0.0};
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < rows; r += kFinishThreads) {
+    float w;
+    row_token(idx, r, vocab, w);
+    x[0] += w;
+  }
+  block_sum(x, s_sum);
+  if (threadIdx.x == 0) *out = x[0];
+}
+
+// Up to this many rows every CTA sums the weights itself; beyond it one block does so first, for all.
+constexpr int64_t kOwnWeights = 2048;
+
 template <typename T>
 cudaError_t launch_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
-                          cudaStream_t stream) {
+                          double* weight_sum, cudaStream_t stream) {
   const PolicyTerms q = *a.policy;
   const auto kern = q.entropy_coef != 0.f ? token_policy_kernel<T, true> : token_policy_kernel<T, false>;
   RowLaunch l = row_launch(a.rows, a.vocab, sizeof(T), true);
   int resident = 0;
-  const cudaError_t e = resident_clusters(kern, l, &resident);
+  cudaError_t e = resident_clusters(kern, l, &resident);
   if (e != cudaSuccess) return e;
   l.clusters = std::min<int64_t>(a.rows, resident);
-  return launch_rows(kern, l, stream, a, q, grad, scale, scale_device, mean, base_of(a.inv_temp));
+  if (!mean || a.rows <= kOwnWeights) weight_sum = nullptr;
+  if (weight_sum != nullptr) {
+    e = launch_pdl(policy_weights_kernel, dim3(1), dim3(kFinishThreads), 0, stream, a.idx, a.rows, a.vocab, weight_sum);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_rows(kern, l, stream, a, q, grad, scale, scale_device, mean, static_cast<const double*>(weight_sum),
+                     base_of(a.inv_temp));
 }
 
 // ---- gradient of the logits from the row statistics -----------------------------------------------------------------------
@@ -826,31 +877,6 @@ cudaError_t launch_grad(const TokenGradArgs& a, cudaStream_t stream) {
 }
 
 // ---- sums over rows, sequences and pairs -----------------------------------------------------------------------------------
-// Sums of a block in fixed order, in every thread. smem: N numbers per warp.
-template <int N>
-__device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    for (int o = 16; o >= 1; o >>= 1) x[n] += __shfl_xor_sync(0xffffffffu, x[n], o);
-  }
-  __syncthreads();
-  if (lane == 0) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) smem[warp * N + n] = x[n];
-  }
-  __syncthreads();
-  if (threadIdx.x < N) {  // fp64 adds are slow: one thread for each sum
-    double y = smem[threadIdx.x];
-    for (int i = 1; i < warps; ++i) y += smem[i * N + threadIdx.x];
-    smem[threadIdx.x] = y;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < N; ++n) x[n] = smem[n];
-}
-
-constexpr int kFinishThreads = 1024;
 __global__ void __launch_bounds__(kFinishThreads) policy_finish_kernel(const PolicyFinishArgs a) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
@@ -1013,12 +1039,12 @@ cudaError_t token_stats(const TokenStatsArgs& a, cudaStream_t stream) {
 }
 
 cudaError_t token_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
-                         cudaStream_t stream) {
+                         double* weight_sum, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
   switch (a.dtype) {
-    case kTokF32: return launch_policy<float>(a, grad, scale, scale_device, mean, stream);
-    case kTokBF16: return launch_policy<__nv_bfloat16>(a, grad, scale, scale_device, mean, stream);
-    default: return launch_policy<__half>(a, grad, scale, scale_device, mean, stream);
+    case kTokF32: return launch_policy<float>(a, grad, scale, scale_device, mean, weight_sum, stream);
+    case kTokBF16: return launch_policy<__nv_bfloat16>(a, grad, scale, scale_device, mean, weight_sum, stream);
+    default: return launch_policy<__half>(a, grad, scale, scale_device, mean, weight_sum, stream);
   }
 }
 

@@ -52,9 +52,9 @@ struct TokenStatsArgs {
 cudaError_t token_stats(const TokenStatsArgs& a, cudaStream_t stream);
 // The statistics with `policy` and the gradient times scale (times *scale_device) in one pass; with `mean` the gradient is
 // divided by the sum of the weights. `grad` rows start at the same places within 16 bytes as the logits' rows. Writes logp
-// and terms.
+// and terms. weight_sum: room for one number.
 cudaError_t token_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
-                         cudaStream_t stream);
+                         double* weight_sum, cudaStream_t stream);
 
 struct TokenGradArgs {
   int dtype;

@@ -88,8 +88,8 @@ def _check_cpu(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | 
             raise ValueError(f"{name} must be on the device of the logits")
         if x.shape != logits.shape[:-1]:
             raise ValueError(f"{name} must have the shape {tuple(logits.shape[:-1])}, got {tuple(x.shape)}")
-    if not (math.isfinite(temperature) and temperature > 0.0):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must lie in [1e-6, 1e6], got {temperature}")
 
 
 # ---- log-probabilities ----------------------------------------------------------------------------------------------------
