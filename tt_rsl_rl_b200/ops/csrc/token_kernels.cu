@@ -494,7 +494,8 @@ __device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ra
 
 // ---- row statistics -----------------------------------------------------------------------------------------------------
 // A CTA per row, or a cluster of them where rows are few: each CTA a share of the row's vectors, whose sums meet in every
-// CTA's shared memory.
+// CTA's shared memory. Bound by memory for fp32 (737 MB in 116 us, 97 % of the copy rate); for bf16 by the instructions of
+// a column too (one ex2 of the special-function unit, about seven others): 268 MB in 60 us, 2.1 GB in 316 us (95 %).
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                       bool policy, const Base k) {
@@ -566,7 +567,11 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
 }
 
 // A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
-// the rows in work fit L2 (row_ranks), so the logits come from memory once.
+// the rows in work fit L2 (row_launch), and loads that say which read is the last keep them there. Measured at 8,192 rows
+// of 131,072 bf16 columns (a tenth masked): 891 us, where statistics and gradient as two kernels take 316 + 663; memory
+// traffic is 1.15 times one read and one write, so most second reads hit. What remains is the latency between the two
+// halves of a row (warps wait for loads 5 of 14 cycles). The row held in shared memory behind bulk copies, its clusters of
+// 8 exchanging sums, took 1,016 us: an exchange costs 2 us a row.
 template <typename T, bool kEnt>
 __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                        const TokenRows grad, float scale,
@@ -679,18 +684,25 @@ struct RowLaunch {
   int64_t clusters;
 };
 
+// A launch without clusters says nothing of them: with a cluster dimension of one the kernels above ran up to 2.4 times
+// slower for short rows (65,536 rows of 1,024 columns: 168 us against 69).
 cudaLaunchConfig_t row_config(const RowLaunch& l, cudaStream_t stream, cudaLaunchAttribute (&attr)[2]) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(l.clusters * l.ranks));
   cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
   cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(l.ranks);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (l.ranks > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(l.ranks);
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   return cfg;
 }
 
@@ -714,12 +726,16 @@ cudaError_t resident_clusters(Kern kern, const RowLaunch& l, int* count) {
       return cudaSuccess;
     }
   }
-  cudaLaunchAttribute attr[2];
-  RowLaunch one = l;
-  one.clusters = 1;
-  cudaLaunchConfig_t cfg = row_config(one, nullptr, attr);
-  cfg.numAttrs = 1;
-  e = cudaOccupancyMaxActiveClusters(count, kern, &cfg);
+  if (l.ranks == 1) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(count, kern, l.threads, 0);
+    *count *= sm_count();
+  } else {
+    cudaLaunchAttribute attr[2];
+    RowLaunch one = l;
+    one.clusters = 1;
+    const cudaLaunchConfig_t cfg = row_config(one, nullptr, attr);
+    e = cudaOccupancyMaxActiveClusters(count, kern, &cfg);
+  }
   if (e != cudaSuccess) return e;
   *count = std::max(*count, 1);
   known.push_back({reinterpret_cast<const void*>(kern), device, l.ranks, l.threads, *count});
@@ -733,9 +749,13 @@ cudaError_t launch_rows(void (*kern)(KArgs...), const RowLaunch& l, cudaStream_t
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// Threads of a CTA: eight vectors each, 32 to 256. CTAs of a row: as many as leave every thread a vector while all rows
-// together stay within one wave; and with `again` (the row is read a second time) as many as keep the rows of a wave
-// within `kCached` bytes.
+// Threads of a CTA: eight vectors each, 32 to 256 (four CTAs of 256 hide a row's end behind other rows: 4,094 rows of 50,001
+// fp32 columns took 116 us, with 512 threads 126, with 1,024 201).
+// CTAs of a row: where rows are few, as many as stay within one wave and leave a thread four vectors or more (fewer are
+// not worth the exchange: 1,024 rows of 1,024 bf16 columns 3.4 us unsplit, 12.7 in clusters of 4; 4 rows of 131,072 take
+// 4.5 us in clusters of 8). With `again` (the row is read a second time) as many as keep the rows of a wave within
+// `kCached` bytes of the 126 MB of L2 (8,192 rows of 131,072 bf16 columns: 893 us at 110 MB, 891 at 80, 931 at 60, 1,111
+// at 32, where clusters of 8 wait for each other).
 constexpr int64_t kCached = 80 << 20;
 RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again) {
   const int64_t sms = sm_count(), nvec = vocab * size / 16;
@@ -743,7 +763,7 @@ RowLaunch row_launch(int64_t rows, int64_t vocab, int size, bool again) {
   l.threads = static_cast<int>(std::min<int64_t>(kMostThreads, std::max<int64_t>(32, (nvec / 8 + 31) / 32 * 32)));
   const int64_t resident = std::min<int64_t>(1024 / l.threads, 32) * sms;
   l.ranks = 1;
-  while (l.ranks < kMaxCluster && nvec >= 2 * l.ranks * l.threads) {
+  while (l.ranks < kMaxCluster && nvec >= 8 * l.ranks * l.threads) {
     const bool idle = rows * l.ranks * 2 <= resident;
     const bool large = again && std::min(rows, resident / l.ranks) * vocab * size > kCached;
     if (!idle && !large) break;
@@ -778,8 +798,9 @@ __global__ void __launch_bounds__(kFinishThreads) policy_weights_kernel(const To
   if (threadIdx.x == 0) *out = x[0];
 }
 
-// Up to this many rows every CTA sums the weights itself; beyond it one block does so first, for all.
-constexpr int64_t kOwnWeights = 2048;
+// Up to this many rows every CTA sums the weights itself; beyond it one block does so first, for all (whole call, own sum
+// against one block's: 1,024 rows of 16,384 columns 21.5 against 22.6 us; 4,096 of 1,024 25.3 against 20.1).
+constexpr int64_t kOwnWeights = 1024;
 
 template <typename T>
 cudaError_t launch_policy(const TokenStatsArgs& a, const TokenRows& grad, float scale, const float* scale_device, int mean,
@@ -805,7 +826,7 @@ constexpr int kGradThreads = 256;
 constexpr int kGradVecs = 8;  // vectors per thread
 
 // A block writes one row's segment of 16-byte vectors. Rows run backwards: the last ones that the statistics read are
-// still in L2.
+// still in L2. Bound by memory: 268 MB read and written in 84 us (6.4 TB/s, 98 % of the copy rate).
 template <typename T, bool kEnt>
 __global__ void __launch_bounds__(kGradThreads) token_grad_kernel(const TokenGradArgs a, int segs, const Base k) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
@@ -921,7 +942,7 @@ __device__ __forceinline__ float softplus_neg(float x) { return log1pf(expf(-fab
 constexpr int kPairThreads = 1024;
 // One block, split into teams of threads: a team sums the log-probabilities of a pair's two sequences (in 64 bits, in a
 // fixed order), its first thread works out the pair's loss, and the team writes the rows' coefficients. Tens of thousands
-// of rows are a few hundred kilobytes, so one block's time stays far below the logits'.
+// of rows are a few hundred kilobytes, so one block's time stays far below the logits' (8,000 rows: 12 us beside 430).
 __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const PreferenceArgs a) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
