@@ -331,6 +331,29 @@ def test_autograd_twice_and_same_as_grad_form():
         assert token_policy_loss(z, tokens, old, adv, mask=mask).loss.item() == pytest.approx(loss.item(), abs=1e-6)
 
 
+def test_differentiable_once():
+    x, tokens, old, adv, mask = _inputs(8, 8, 100)
+    z = x.float().requires_grad_()
+    for value in (token_logprobs(z, tokens)[0].sum(), token_policy_loss(z, tokens, old, adv).loss,
+                  preference_loss(z, tokens, offsets=torch.tensor([0, 4, 8], device="cuda")).loss):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(value, z, create_graph=True)
+
+
+def test_gradients_reach_leaves_through_views():
+    """The means and log-probabilities of a loss carry no gradient; only one of two outputs may be used."""
+    x, tokens, old, adv, mask = _inputs(9, 8, 100)
+    z = x.float().requires_grad_()
+    out = token_policy_loss(z, tokens, old, adv, mask=mask)
+    assert out.loss.requires_grad and not any(t.requires_grad for t in out[1:])
+    for pick in (0, 1):
+        z.grad = None
+        token_logprobs(z, tokens)[pick].sum().backward()
+        assert torch.isfinite(z.grad).all() and z.grad.abs().sum() > 0
+    pref = preference_loss(z.view(2, 4, 100), tokens.view(2, 4))
+    assert pref.loss.requires_grad and not any(t.requires_grad for t in pref[1:])
+
+
 def test_scale_on_the_device():
     x, tokens, old, adv, mask = _inputs(6)
     _, one = token_policy_loss_grad(x, tokens, old, adv, grad_scale=8.0)

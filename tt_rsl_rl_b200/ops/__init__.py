@@ -20,9 +20,9 @@ _PROFILER: profile_ops | None = None
 LAUNCHING = frozenset({
     "adam_step", "adamw_step", "adv_gather_stats", "adv_normalize", "colstats", "counter_add", "gae", "gather_minibatch",
     "gaussian_sample", "gemm", "lg_env_step", "mse_grad", "norm_update", "p2p_allreduce_f64", "p2p_broadcast_f32",
-    "ppo_loss", "preference_loss", "prep_obs", "process_step", "reduce_segments", "rnd_intrinsic", "rnd_reward_scale",
-    "rnn_cell_bwd", "rnn_cell_fwd", "rnn_mask", "to_bf16_padded", "token_logprobs", "token_logprobs_backward",
-    "token_loss_backward", "token_policy_loss",
+    "ppo_loss", "preference_loss", "preference_loss_autograd", "prep_obs", "process_step", "reduce_segments",
+    "rnd_intrinsic", "rnd_reward_scale", "rnn_cell_bwd", "rnn_cell_fwd", "rnn_mask", "to_bf16_padded", "token_logprobs",
+    "token_logprobs_autograd", "token_policy_loss", "token_policy_loss_autograd",
 })
 
 

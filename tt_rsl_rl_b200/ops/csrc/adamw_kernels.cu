@@ -127,8 +127,9 @@ __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
 // Sum of squares with its rounding errors: s + e is right to about 2^-45, so the norm in fp32 does not depend on the order
-// of the sum, at fp32 speed: summing in fp64 took 648 us for 335 M bf16 gradients, this 150 (4.5 TB/s). T. J. Dekker, "A floating-point technique for extending the available
-// precision" (1971): the error of s + x is x - ((s + x) - s) where s is the larger; a sum of squares outgrows its terms.
+// of the sum, at fp32 speed: summing in fp64 took 648 us for 335 M bf16 gradients, this 150 (4.5 TB/s). T. J. Dekker, "A
+// floating-point technique for extending the available precision" (1971): the error of s + x is x - ((s + x) - s) where s
+// is the larger; a sum of squares outgrows its terms.
 struct SquareSum {
   float s = 0.f, e = 0.f;
   template <bool kExact>  // kExact: x * x fits fp32 (bf16 gradients)
@@ -240,7 +241,9 @@ __device__ __forceinline__ Pair neg2(const Pair& a) { return mul2(a, Pair(-1.f, 
 __device__ __forceinline__ void sqrt2(const float (&v)[2], float (&r)[2]) {
   float y[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) asm("rsqrt.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(fmaxf(v[i], __int_as_float(1))));  // zero stays zero below
+  for (int i = 0; i < 2; ++i) {  // from the smallest number up: zero stays zero below
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(y[i]) : "f"(fmaxf(v[i], __int_as_float(1))));
+  }
   const Pair x(v[0], v[1]), y2(y[0], y[1]), half(0.5f, 0.5f);
   Pair g = mul2(x, y2), h = mul2(y2, half);
   const Pair e = fma2(neg2(h), g, half);

@@ -2,6 +2,7 @@
 // types, shapes and strides, then launches on the current stream of the tensors' device; scratch memory comes from the
 // caching allocator of that stream, call by call.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -351,6 +352,103 @@ std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, 
   return result;
 }
 
+// ---- differentiable forms -----------------------------------------------------------------------------------------------
+// Autograd in C++: a backward pass in Python waits for the interpreter (log-probabilities and their gradient for a few rows
+// took 84 us, these 61). They keep the logits and a few numbers per row.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void backward_checks(const char* name) {
+  TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, name,
+              ": a backward pass cannot be captured in a CUDA graph; capture a form that returns the gradient");
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once (create_graph is not supported)");
+}
+
+Tensor or_none(const OptT& t) { return given(t) ? *t : Tensor(); }
+OptT optional(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+
+struct LogProbs : torch::autograd::Function<LogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const OptT& mask,
+                               double temperature) {
+    const std::vector<Tensor> x = token_logprobs(logits, tokens, mask, temperature);  // logp, entropy, ml
+    ctx->save_for_backward({logits, tokens, or_none(mask), x[2], x[1]});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->set_materialize_grads(false);
+    return {x[0], x[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& d) {
+    backward_checks("token_logprobs");
+    if (!d[0].defined() && !d[1].defined()) return variable_list(4);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor d_logp = d[0].defined() ? d[0] : torch::zeros_like(d[1]);
+    return {token_logprobs_backward(s[0], s[1], optional(s[2]), ctx->saved_data["temperature"].toDouble(), s[3], s[4],
+                                    d_logp, optional(d[1])),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct PolicySettings {
+  double clip_lo, clip_hi, kl_coef;
+  int64_t kl_kind;
+  double entropy_coef, temperature;
+  bool mean;
+};
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const Tensor& old,
+                               const Tensor& adv, const OptT& ref, const OptT& mask, const PolicySettings& p) {
+    // loss, four means, factor, logp, entropy, ml, coef
+    const std::vector<Tensor> x =
+        token_policy_loss(logits, tokens, old, adv, ref, mask, p.clip_lo, p.clip_hi, p.kl_coef, p.kl_kind,
+                          p.entropy_coef, p.temperature, p.mean, false, 1.0, OptT());
+    ctx->save_for_backward(
+        {logits, tokens, or_none(mask), x[8], p.entropy_coef != 0.0 ? x[7] : Tensor(), x[9], x[5]});
+    ctx->saved_data["temperature"] = p.temperature;
+    ctx->mark_non_differentiable({x[1], x[2], x[3], x[4], x[6]});
+    ctx->set_materialize_grads(false);
+    return {x[0], x[1], x[2], x[3], x[4], x[6]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& d) {
+    backward_checks("token_policy_loss");
+    if (!d[0].defined()) return variable_list(7);
+    const variable_list s = ctx->get_saved_variables();
+    variable_list grads(7);
+    grads[0] = token_loss_backward(s[0], s[1], optional(s[2]), ctx->saved_data["temperature"].toDouble(), s[3],
+                                   optional(s[4]), s[5], s[6], d[0]);
+    return grads;
+  }
+};
+
+struct PreferenceSettings {
+  double beta, smoothing;
+  int64_t kind;
+  bool average;
+  double temperature;
+};
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, const OptT& ref,
+                               const OptT& offsets, const OptT& mask, const PreferenceSettings& p) {
+    // loss, two rewards, seq_logp, logp, ml, coef
+    const std::vector<Tensor> x = preference_loss(logits, tokens, ref, offsets, mask, p.beta, p.smoothing, p.kind,
+                                                  p.average, p.temperature, false, 1.0, OptT());
+    ctx->save_for_backward({logits, tokens, or_none(mask), x[5], x[6]});
+    ctx->saved_data["temperature"] = p.temperature;
+    ctx->mark_non_differentiable({x[1], x[2], x[3], x[4]});
+    ctx->set_materialize_grads(false);
+    return {x[0], x[1], x[2], x[3], x[4]};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& d) {
+    backward_checks("preference_loss");
+    if (!d[0].defined()) return variable_list(6);
+    const variable_list s = ctx->get_saved_variables();
+    variable_list grads(6);
+    grads[0] = token_loss_backward(s[0], s[1], optional(s[2]), ctx->saved_data["temperature"].toDouble(), s[3], OptT(),
+                                   s[4], OptT(), d[0]);
+    return grads;
+  }
+};
+
 // ---- AdamW ------------------------------------------------------------------------------------------------------------
 // The parameters and states of one step over many tensors. Holds the tensors; pointers are read at every step.
 class AdamWPlan {
@@ -540,9 +638,23 @@ OptT adamw_step(const std::vector<AdamWPlan*>& plans, const std::vector<AdamSett
 
 void rlb_register_token(pybind11::module& m) {
   m.def("token_logprobs", &token_logprobs);
-  m.def("token_logprobs_backward", &token_logprobs_backward);
   m.def("token_policy_loss", &token_policy_loss);
-  m.def("token_loss_backward", &token_loss_backward);
+  m.def("token_logprobs_autograd", [](const Tensor& logits, const Tensor& tokens, const OptT& mask, double temperature) {
+    return LogProbs::apply(logits, tokens, mask, temperature);
+  });
+  m.def("token_policy_loss_autograd",
+        [](const Tensor& logits, const Tensor& tokens, const Tensor& old, const Tensor& adv, const OptT& ref,
+           const OptT& mask, double clip_lo, double clip_hi, double kl_coef, int64_t kl_kind, double entropy_coef,
+           double temperature, bool mean) {
+          return PolicyLoss::apply(logits, tokens, old, adv, ref, mask,
+                                   PolicySettings{clip_lo, clip_hi, kl_coef, kl_kind, entropy_coef, temperature, mean});
+        });
+  m.def("preference_loss_autograd",
+        [](const Tensor& logits, const Tensor& tokens, const OptT& ref, const OptT& offsets, const OptT& mask, double beta,
+           double smoothing, int64_t kind, bool average, double temperature) {
+          return PreferenceLoss::apply(logits, tokens, ref, offsets, mask,
+                                       PreferenceSettings{beta, smoothing, kind, average, temperature});
+        });
   m.def("preference_loss", &preference_loss);
   m.attr("adamw_block") = rlb::kAdamBlock;
   pybind11::class_<AdamWPlan>(m, "AdamWPlan")

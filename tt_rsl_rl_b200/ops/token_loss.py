@@ -111,28 +111,6 @@ def _logprobs_torch(logits, tokens, weights, temperature):
     return torch.where(counted, logp, 0.0), torch.where(counted, entropy, 0.0)
 
 
-class _LogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, mask, temperature):
-        logp, entropy, stats = ext().token_logprobs(logits, tokens, mask, temperature)
-        ctx.save_for_backward(logits, tokens, mask, stats, entropy)
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
-        return logp, entropy
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_logp, d_entropy):
-        _refuse_capture("token_logprobs")
-        if d_logp is None and d_entropy is None:
-            return None, None, None, None
-        logits, tokens, mask, stats, entropy = ctx.saved_tensors
-        if d_logp is None:
-            d_logp = torch.zeros_like(d_entropy)
-        return ext().token_logprobs_backward(logits, tokens, mask, ctx.temperature, stats, entropy, d_logp,
-                                             d_entropy), None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Tensor | None = None,
                    temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """``(logp, entropy)`` of each row, float32: the log-probability of its token under
@@ -142,7 +120,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Te
         return _logprobs_torch(logits, tokens, _row_weights(logits, tokens, mask), temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_capture("token_logprobs")
-        return _LogProbs.apply(logits, tokens, mask, temperature)
+        return tuple(ext().token_logprobs_autograd(logits, tokens, mask, temperature))
     logp, entropy, _ = ext().token_logprobs(logits, tokens, mask, temperature)
     return logp, entropy
 
@@ -190,27 +168,6 @@ def _policy_torch(logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind,
     return TokenPolicyLoss((loss * inv if mean else loss).float(), *stats, logp.detach())
 
 
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, old, adv, ref, mask, settings, temperature):
-        lo, hi, kl_coef, kl_kind, entropy_coef, mean = settings
-        loss, *means, factor, logp, entropy, stats, coef = ext().token_policy_loss(
-            logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind, entropy_coef, temperature, mean, False, 1.0,
-            None)
-        ctx.save_for_backward(logits, tokens, mask, stats, entropy if entropy_coef != 0.0 else None, coef, factor)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(*means, logp)
-        return loss, *means, logp
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, *_):
-        _refuse_capture("token_policy_loss")
-        logits, tokens, mask, stats, entropy, coef, factor = ctx.saved_tensors
-        grad = ext().token_loss_backward(logits, tokens, mask, ctx.temperature, stats, entropy, coef, factor, d_loss)
-        return grad, None, None, None, None, None, None, None
-
-
 def token_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
                       ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip_param: float = 0.2,
                       clip_high: float | None = None, kl_coef: float = 0.0, kl_estimator: str = "k3",
@@ -231,8 +188,8 @@ def token_policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torc
         return _policy_torch(logits, tokens, old_logp, advantages, ref_logp, mask, *settings, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_capture("token_policy_loss")
-        return TokenPolicyLoss(*_PolicyLoss.apply(logits, tokens, old_logp, advantages, ref_logp, mask, settings,
-                                                  temperature))
+        return TokenPolicyLoss(*ext().token_policy_loss_autograd(
+            logits, tokens, old_logp, advantages, ref_logp, mask, *settings[:5], temperature, settings[5]))
     parts = ext().token_policy_loss(logits, tokens, old_logp, advantages, ref_logp, mask, *settings[:5], temperature,
                                     settings[5], False, 1.0, None)
     return TokenPolicyLoss(*parts[:5], parts[6])
@@ -327,25 +284,6 @@ def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind,
     return PreferenceLoss(loss, rewards[0::2], rewards[1::2], lp.detach().float(), logp.detach())
 
 
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, ref, offsets, mask, settings, temperature):
-        loss, *parts, stats, coef = ext().preference_loss(logits, tokens, ref, offsets, mask, *settings, temperature,
-                                                          False, 1.0, None)
-        ctx.save_for_backward(logits, tokens, mask, stats, coef)
-        ctx.temperature = temperature
-        ctx.mark_non_differentiable(*parts)
-        return loss, *parts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, *_):
-        _refuse_capture("preference_loss")
-        logits, tokens, mask, stats, coef = ctx.saved_tensors
-        grad = ext().token_loss_backward(logits, tokens, mask, ctx.temperature, stats, None, coef, None, d_loss)
-        return grad, None, None, None, None, None, None
-
-
 def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
                     offsets: torch.Tensor | None = None, mask: torch.Tensor | None = None, beta: float = 0.1,
                     label_smoothing: float = 0.0, loss_type: str = "sigmoid", average: bool = False,
@@ -366,7 +304,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: torch
         return _preference_torch(logits, tokens, ref_logps, offsets, mask, *settings, temperature)
     if logits.requires_grad and torch.is_grad_enabled():
         _refuse_capture("preference_loss")
-        return PreferenceLoss(*_PreferenceLoss.apply(logits, tokens, ref_logps, offsets, mask, settings, temperature))
+        return PreferenceLoss(*ext().preference_loss_autograd(logits, tokens, ref_logps, offsets, mask, *settings,
+                                                              temperature))
     parts = ext().preference_loss(logits, tokens, ref_logps, offsets, mask, *settings, temperature, False, 1.0, None)
     return PreferenceLoss(*parts[:5])
 
