@@ -429,7 +429,7 @@ struct Quad {
 // A warp takes units of 256 elements: lane l elements [4 l, 4 l + 4) and [128 + 4 l, ...), so every access of the warp is
 // contiguous. The unit is also the block of a scale, whose maximum is a warp reduction. With 32-bit states the step is
 // bound by memory; with 8-bit states by its instructions, about 110 an element (random numbers, both roundings, root and
-// quotient): 335 M bf16 weights in 1,506 us, 2.6 times the bytes' time, with 70 % of the issue slots used. Codes taken and
+// quotient): 335 M bf16 weights in 1,501 us, 2.1 times the bytes' time, with 70 % of the issue slots used. Codes taken and
 // packed by shifts and products instead of conversions, and pairs, brought it there from 2,832.
 template <typename T, bool kBits8, int K>
 __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_constant__ AdamTable<K> t,

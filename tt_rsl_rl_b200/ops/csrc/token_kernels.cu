@@ -568,7 +568,7 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
 
 // A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
 // the rows in work fit L2 (row_launch), and loads that say which read is the last keep them there. Measured at 8,192 rows
-// of 131,072 bf16 columns (a tenth masked): 891 us, where statistics and gradient as two kernels take 316 + 663; memory
+// of 131,072 bf16 columns (a tenth masked): 886 us, where statistics and gradient as two kernels take 316 + 663; memory
 // traffic is 1.15 times one read and one write, so most second reads hit. What remains is the latency between the two
 // halves of a row (warps wait for loads 5 of 14 cycles). The row held in shared memory behind bulk copies, its clusters of
 // 8 exchanging sums, took 1,016 us: an exchange costs 2 us a row.
