@@ -212,6 +212,42 @@ def test_resume(dtype, bits):
     resume("cpu", dtype, bits)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_states_of_another_layout(dtype):
+    """32-bit states are laid out anew; the scales of 8-bit ones belong to an order in memory, so those are refused, and
+    so are states of another shape."""
+    torch.manual_seed(2)
+    values, grads = torch.randn(2, 3, 20, 7).to(dtype), [torch.randn(2, 3, 20, 7).to(dtype) for _ in range(2)]
+    p = values.contiguous(memory_format=torch.channels_last).requires_grad_()
+    q = values.clone().requires_grad_()
+    for bits in (32, 8):
+        first, second = AdamW([p], state_bits=bits, **HYPER), AdamW([q], state_bits=bits, **HYPER)
+        p.grad = grads[0]
+        first.step()
+        with torch.no_grad():
+            q.copy_(p)
+        second.load_state_dict(first.state_dict())
+        p.grad, q.grad = grads[1], grads[1]
+        if bits == 8:
+            with pytest.raises(ValueError, match="order in memory"):
+                second.step()
+            continue
+        first.step()
+        second.step()
+        assert torch.equal(p, q)
+        if dtype == torch.bfloat16:
+            assert torch.equal(first.state[p]["low_bits"], second.state[q]["low_bits"])
+    row = torch.ones(7).requires_grad_()
+    third = AdamW([row])
+    wide = AdamW([torch.ones(1).requires_grad_()])
+    wide.param_groups[0]["params"][0].grad = torch.ones(1)
+    wide.step()
+    third.load_state_dict(wide.state_dict())
+    row.grad = torch.ones(7)
+    with pytest.raises(ValueError, match="shape"):
+        third.step()
+
+
 def test_groups_share_the_norm():
     a, b = torch.ones(3).requires_grad_(), torch.ones(4, dtype=torch.bfloat16).requires_grad_()
     opt = AdamW([{"params": [a], "lr": 0.0}, {"params": [b]}], lr=0.1, max_grad_norm=1.0, weight_decay=0.0)

@@ -135,6 +135,11 @@ def _dense(p: torch.Tensor) -> bool:
     return True
 
 
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether tensors of one shape walk memory in the same order (strides of single elements do not matter)."""
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def _flat(x: torch.Tensor) -> torch.Tensor:
     """A dense tensor's elements in memory order (a view)."""
     return x.as_strided((x.numel(),), (1,))
@@ -291,15 +296,23 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if (x.dtype == CODES) != (self.state_bits == 8) or not x.is_floating_point():
                 raise ValueError(f"the loaded {key} is {x.dtype}: it does not belong to {self.state_bits}-bit states")
-            if x.dtype != dtype or x.shape != p.shape or x.stride() != p.stride():
+            if x.shape != p.shape:
+                raise ValueError(f"the loaded {key} has the shape {tuple(x.shape)}, its parameter {tuple(p.shape)}")
+            if self.state_bits == 8 and not _same_order(x, p):
+                raise ValueError(f"the loaded {key} has strides {x.stride()}, its parameter {p.stride()}: the scales of "
+                                 "8-bit states follow the order in memory")
+            if x.dtype != dtype or x.stride() != p.stride():
                 like = torch.empty_like(p, dtype=dtype, memory_format=torch.preserve_format)
                 state[key] = like.copy_(x)
         if self.state_bits == 8:
             for key in ("exp_avg_scale", "exp_avg_sq_scale"):
                 if state.get(key) is None:
                     state[key] = torch.zeros(-(-p.numel() // BLOCK), device=p.device)
-        if p.dtype == torch.bfloat16 and state.get("low_bits") is None:
-            state["low_bits"] = torch.zeros_like(p, dtype=torch.int16, memory_format=torch.preserve_format)
+        if p.dtype == torch.bfloat16:
+            low = state.get("low_bits")
+            if low is None or (low.dtype == torch.int16 and low.shape == p.shape and low.stride() != p.stride()):
+                like = torch.zeros_like(p, dtype=torch.int16, memory_format=torch.preserve_format)
+                state["low_bits"] = like if low is None else like.copy_(low)
         return state
 
     def _build(self) -> list[tuple[dict, AdamWPlan]]:
