@@ -248,6 +248,33 @@ def test_states_of_another_layout(dtype):
         third.step()
 
 
+def test_states_of_another_update():
+    """What AdamW's step would leave out is refused when it is loaded; groups of older dictionaries lack settings."""
+    p = torch.ones(5).requires_grad_()
+    p.grad = torch.ones(5)
+    theirs = torch.optim.AdamW([p], amsgrad=True)
+    theirs.step()
+    with pytest.raises(ValueError, match="amsgrad"):
+        AdamW([p]).load_state_dict(theirs.state_dict())
+    theirs = torch.optim.Adam([p], weight_decay=0.1)
+    theirs.step()
+    with pytest.raises(ValueError, match="decoupled"):
+        AdamW([p]).load_state_dict(theirs.state_dict())
+    theirs = torch.optim.Adam([p])
+    theirs.step()
+    state = theirs.state_dict()
+    del state["param_groups"][0]["maximize"]
+    ours = AdamW([p])
+    ours.load_state_dict(state)
+    q = p.detach().clone().requires_grad_()
+    q.grad = p.grad.clone()
+    again = torch.optim.Adam([q])
+    again.load_state_dict(theirs.state_dict())
+    ours.step()
+    again.step()
+    assert torch.allclose(p, q, atol=1e-6)
+
+
 def test_groups_share_the_norm():
     a, b = torch.ones(3).requires_grad_(), torch.ones(4, dtype=torch.bfloat16).requires_grad_()
     opt = AdamW([{"params": [a], "lr": 0.0}, {"params": [b]}], lr=0.1, max_grad_norm=1.0, weight_decay=0.0)

@@ -248,7 +248,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits``: 32 or 8. ``max_grad_norm``: clip the global gradient norm inside the step (``grad_norm`` holds the
     norm afterwards). Parameters are float32 or bfloat16, all on one device. In a 32-bit optimizer, state dictionaries
-    of ``torch.optim.AdamW`` load."""
+    of ``torch.optim.AdamW`` load. The tensors of ``state`` and the lists of parameters are bound at the first step:
+    write states in place or load a state dictionary, add parameters with ``add_param_group``."""
 
     def __init__(self, params, lr: float | torch.Tensor = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: float | None = None,
@@ -268,6 +269,8 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("maximize", False)
         self._plans, self.grad_norm = None, None
 
     def add_param_group(self, param_group) -> None:
@@ -276,6 +279,11 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """The base class casts states to the parameter's type; codes, scales and float32 moments keep theirs here."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad"):
+                raise ValueError("AdamW: the loaded state is of an update with amsgrad, which this one has not")
+            if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0.0) != 0.0:
+                raise ValueError("AdamW: the loaded state is of an update whose weight decay is not decoupled")
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         super().load_state_dict(state_dict)
         own = [p for group in self.param_groups for p in group["params"]]
