@@ -499,11 +499,13 @@ __device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ra
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                       bool policy, const Base k) {
-  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
-  griddep_launch_dependents();
   __shared__ RowExchange x;
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  if (ranks > 1) cluster.barrier_arrive();  // no CTA writes into another before that one has started
+  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
+  griddep_launch_dependents();
+  if (ranks > 1) cluster.barrier_wait();
   int parity = 0;
   for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
     float w;
@@ -577,14 +579,15 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
                                                                        const TokenRows grad, float scale,
                                                                        const float* scale_device, int mean,
                                                                        const double* weight_sum, const Base k) {
-  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
-  griddep_launch_dependents();
   constexpr int VN = Elem<T>::kPerVec;
   __shared__ RowExchange x;
   __shared__ double s_sum[kMostWarps];
   __shared__ RowGrad s_grad[2];
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  if (ranks > 1) cluster.barrier_arrive();  // no CTA writes into another before that one has started
+  griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
+  griddep_launch_dependents();
   const int threads = blockDim.x;
   if (scale_device) scale *= *scale_device;
   if (mean) {
@@ -602,6 +605,7 @@ __global__ void __launch_bounds__(kMostThreads, 4) token_policy_kernel(const Tok
     scale *= total[0] != 0.0 ? static_cast<float>(1.0 / total[0]) : 0.f;
   }
   const float factor = scale * k.inv;
+  if (ranks > 1) cluster.barrier_wait();
   int parity = 0;
   for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
     float w;
