@@ -354,6 +354,22 @@ def test_gradients_reach_leaves_through_views():
     assert pref.loss.requires_grad and not any(t.requires_grad for t in pref[1:])
 
 
+@pytest.mark.parametrize("estimator", ["k1", "k2", "k3"])
+def test_infinite_divergence_without_weight(estimator):
+    """A reference that excludes a token makes the divergence infinite; with kl_coef 0 the loss does not see it."""
+    x, tokens, old, adv, mask = _inputs(10)
+    ref = old.clone()
+    ref[mask.nonzero()[0]] = float("-inf")
+    args = (x, tokens, old, adv)
+    plain, grad = token_policy_loss_grad(*args, mask=mask)
+    out, with_ref = token_policy_loss_grad(*args, ref_logp=ref, mask=mask, kl_estimator=estimator)
+    assert not torch.isfinite(out.kl) and torch.equal(out.loss, plain.loss) and torch.equal(with_ref, grad)
+    z = x.clone().requires_grad_()
+    loss = token_policy_loss(z, tokens, old, adv, ref_logp=ref, mask=mask, kl_estimator=estimator).loss
+    loss.backward()
+    assert torch.equal(loss.detach(), plain.loss) and torch.isfinite(z.grad).all()
+
+
 def test_scale_on_the_device():
     x, tokens, old, adv, mask = _inputs(6)
     _, one = token_policy_loss_grad(x, tokens, old, adv, grad_scale=8.0)

@@ -2,7 +2,7 @@
 // uploaded or kept between calls and a captured step stays valid as long as its tensors do.
 //
 // Every operation is rounded on its own (no fused multiply-add), as the same expression written with tensor operations
-// rounds it, and the norm is summed in 64 bits in a fixed order: the step does not depend on how tensors are split.
+// rounds it, and the norm is summed together with its rounding errors: the step does not depend on how tensors are split.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 

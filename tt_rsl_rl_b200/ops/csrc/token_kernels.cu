@@ -927,7 +927,8 @@ __global__ void __launch_bounds__(kFinishThreads) policy_finish_kernel(const Pol
   if (threadIdx.x == 0) {
     const double inv = x[4] != 0.0 ? 1.0 / x[4] : 0.0;  // no row counts: loss and gradients are zero
     const double f = a.mean ? inv : 1.0;
-    a.loss[0] = static_cast<float>(f * (x[0] + a.kl_coef * x[1] - a.entropy_coef * x[2]));
+    const double kl = a.kl_coef != 0.f ? a.kl_coef * x[1] : 0.0;  // a divergence without a weight may be infinite
+    a.loss[0] = static_cast<float>(f * (x[0] + kl - a.entropy_coef * x[2]));
     for (int n = 0; n < 4; ++n) a.out[n] = static_cast<float>(inv * x[n]);
     a.out[4] = static_cast<float>(f);
   }
