@@ -389,3 +389,19 @@ def test_preference_refusals():
     x, tokens, old, adv, mask = _inputs(7, 8, 100)
     with pytest.raises(ValueError, match="device"):
         token_logprobs(x, tokens.cpu())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_logprobs_weights_only_select(dtype):
+    """A float mask decides which rows count; neither the log-probabilities nor their gradients are weighted by it."""
+    x, tokens, mask, g = _make((40,), 1001, dtype, seed=11)
+    w = torch.where(mask, torch.linspace(-2.0, 3.0, 40), 0.0)
+    a, b = torch.randn(40, generator=g), torch.randn(40, generator=g) * 0.3
+    for how in ("plain", "offset"):
+        z = _place(x, how).requires_grad_()
+        logp, entropy = token_logprobs(z, tokens.cuda(), mask=w.cuda())
+        _, want, _ = oracle.rows(x, tokens, mask, 1.0)
+        want = torch.where(mask, want, 0.0)
+        assert ((logp.detach().double().cpu() - want).abs() <= oracle.logp_bound(want)).all()
+        grad, = torch.autograd.grad((logp, entropy), z, (a.cuda(), b.cuda()))
+        _check_grad(grad, x, tokens, mask, 1.0, a.double(), b.double())

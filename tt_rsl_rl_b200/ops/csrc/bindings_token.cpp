@@ -172,7 +172,6 @@ Tensor token_logprobs_backward(const Tensor& logits, const Tensor& tokens, const
     db = l.row_input(*d_entropy, "d_entropy", torch::kFloat32);
     a.b = db.data_ptr<float>(), a.b_stride = 1;
   }
-  a.weighted = 0;
   a.scale = 1.f;
   ok(rlb::token_grad(a, at::cuda::getCurrentCUDAStream()), "token_logprobs_backward");
   return grad;
@@ -247,8 +246,7 @@ std::vector<Tensor> token_policy_loss(const Tensor& logits, const Tensor& tokens
     g.ml = a.ml, g.entropy = a.entropy;
     g.a = coef.data_ptr<float>(), g.a_stride = 2;
     if (q.entropy_coef != 0.f) g.b = coef.data_ptr<float>() + 1, g.b_stride = 2;
-    g.weighted = 1;
-    g.scale = static_cast<float>(grad_scale), g.scale_a = scale_device;
+      g.scale = static_cast<float>(grad_scale), g.scale_a = scale_device;
     g.scale_b = out.data_ptr<float>() + 5;
     ok(rlb::token_grad(g, stream), "token_policy_loss");
   }
@@ -277,7 +275,6 @@ Tensor token_loss_backward(const Tensor& logits, const Tensor& tokens, const Opt
     g.entropy = entropy->data_ptr<float>();
     g.b = g.a + 1, g.b_stride = width;
   }
-  g.weighted = 1;
   g.scale = 1.f, g.scale_a = scale_ptr(l, grad_output), g.scale_b = scale_ptr(l, factor);
   ok(rlb::token_grad(g, at::cuda::getCurrentCUDAStream()), "token_loss_backward");
   return grad;
@@ -345,7 +342,6 @@ std::vector<Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, 
   g.out = Logits::rows_of(grad);
   g.ml = a.ml;
   g.a = p.coef, g.a_stride = 1;
-  g.weighted = 1;
   g.scale = static_cast<float>(grad_scale), g.scale_a = scale_ptr(l, grad_scale_device);
   ok(rlb::token_grad(g, stream), "preference_loss");
   result.push_back(grad);

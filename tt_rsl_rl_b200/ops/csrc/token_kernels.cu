@@ -850,7 +850,6 @@ __global__ void __launch_bounds__(kGradThreads) token_grad_kernel(const TokenGra
     float f = static_cast<float>(a.scale * a.inv_temp);
     if (a.scale_a) f *= *a.scale_a;
     if (a.scale_b) f *= *a.scale_b;
-    if (!a.weighted) f *= w;
     ca = a.a[row * a.a_stride] * f;
     if (kEnt) cb = a.b[row * a.b_stride] * f;
   }

@@ -64,9 +64,8 @@ struct TokenGradArgs {
   double inv_temp;
   const float2* ml;
   const float* entropy;  // needed where b is given
-  const float *a, *b;    // dL/dlogp and dL/dH of row r at a[r * a_stride]; b may be null (no entropy term)
+  const float *a, *b;    // dL/dlogp and dL/dH of row r at a[r * a_stride], weights included; b may be null (no entropy term)
   int64_t a_stride, b_stride;
-  int weighted;          // 1: a and b already hold the rows' weights, 0: they are multiplied by them here
   float scale;
   const float *scale_a, *scale_b;  // optional factors on the device
 };

@@ -114,7 +114,8 @@ def _logprobs_torch(logits, tokens, weights, temperature):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Tensor | None = None,
                    temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """``(logp, entropy)`` of each row, float32: the log-probability of its token under
-    ``softmax(logits / temperature)`` and that distribution's entropy. Differentiable by the logits."""
+    ``softmax(logits / temperature)`` and that distribution's entropy. Differentiable by the logits. ``mask`` only says
+    which rows count: a float mask weighs neither the results nor their gradients."""
     if not logits.is_cuda:
         _check_cpu(logits, tokens, mask, temperature)
         return _logprobs_torch(logits, tokens, _row_weights(logits, tokens, mask), temperature)
