@@ -179,3 +179,24 @@ def refuse_preference(device):
 
 def test_preference_refusals():
     refuse_preference("cpu")
+
+
+def extreme_rows(dtype, top, vocab, seed=0):
+    """Eight rows whose largest logits lie within six steps of their type around ``top``: at every column; on every column
+    but one; at a tenth of the columns beside far lower ones, -inf and the type's lowest value; all equal; ordinary logits
+    with a tenth of the columns at ``top`` where that is low. And the column of each row's largest logit."""
+    g = torch.Generator().manual_seed(seed)
+    bits = {4: torch.int32, 2: torch.int16}[dtype.itemsize]
+    near = torch.full((8, vocab), top, dtype=torch.float64).to(dtype)
+    near = (near.view(bits) + torch.randint(-6, 7, near.shape, generator=g).to(bits)).view(dtype)
+    x = near.clone()
+    x[1, vocab // 2] = near[1].max()
+    few = torch.rand(vocab, generator=g) < 0.1
+    few[vocab // 3] = True
+    x[2] = torch.where(few, near[2], float("-inf"))
+    x[3] = torch.where(few, near[3], torch.finfo(dtype).min)
+    x[4] = torch.where(few, near[4], (near[4].double() - abs(top) / 2).to(dtype))
+    x[5] = x[5, 0]
+    ordinary = (torch.randn(2, vocab, generator=g) * 3).to(dtype)
+    x[6:] = torch.where(few & (near[6:] < ordinary), near[6:], ordinary)
+    return x, x.double().argmax(-1)

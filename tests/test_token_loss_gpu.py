@@ -1,10 +1,12 @@
 """Token-policy kernels against 64-bit definitions: types, vocabularies, strides, masks, extremes, capture, streams."""
 
+import math
+
 import pytest
 import torch
 
 import token_oracle as oracle
-from test_token_loss import REFUSALS, refuse, refuse_preference
+from test_token_loss import REFUSALS, extreme_rows, refuse, refuse_preference
 from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
                                            token_policy_loss_grad)
 
@@ -405,3 +407,58 @@ def test_logprobs_weights_only_select(dtype):
         assert ((logp.detach().double().cpu() - want).abs() <= oracle.logp_bound(want)).all()
         grad, = torch.autograd.grad((logp, entropy), z, (a.cuda(), b.cuda()))
         _check_grad(grad, x, tokens, mask, 1.0, a.double(), b.double())
+
+
+def _check_far_grad(got, x, tokens, temperature, a, b, slack=0.0):
+    """``_check_grad`` where probabilities reach below 2^-126 (all rows count). A p is 2^q times a number in [1/2, 2], and
+    2^q below 2^-126 is flushed to zero: that takes p (|a| + |b| (|log p| + H)) / T off an element with p below 2^-125."""
+    counted = torch.ones(tokens.shape, dtype=torch.bool)
+    want, bound = oracle.logits_grad(x, tokens, counted, temperature, a, b)
+    log_p, _, entropy = oracle.rows(x, tokens, counted, temperature)
+    safe = torch.where(log_p == float("-inf"), 0.0, log_p)
+    size = log_p.exp() * (a.abs()[:, None] + b.abs()[:, None] * (safe.abs() + entropy[:, None])) / temperature
+    bound = bound * (1 + slack) + want.abs() * 3e-5 * slack + torch.where(log_p < -125 * math.log(2.0), size, 0.0)
+    assert got.dtype == x.dtype and got.shape == x.shape
+    far = (got.double().cpu() - want).abs() - bound
+    assert (far <= oracle.rounding(want, x.dtype) * 1.01).all(), far.max()
+
+
+def check_extreme(dtype, vocab, temperature, top):
+    """Log-probabilities, entropies, gradients and the policy loss of ``extreme_rows``."""
+    if dtype == torch.float16 and abs(top) > 6e4:
+        return
+    x, best = extreme_rows(dtype, top, vocab)
+    counted = torch.ones(8, dtype=torch.bool)
+    any_token = torch.randint(vocab, (8,), generator=torch.Generator().manual_seed(1))
+    any_token = torch.where(x.gather(1, any_token[:, None])[:, 0] > -3e38 / 4, any_token, best)
+    g = torch.Generator().manual_seed(2)
+    a, b = torch.randn(8, generator=g), torch.randn(8, generator=g) * 0.3
+    for tokens in (best, any_token):
+        z = _place(x, "offset").requires_grad_()
+        logp, entropy = token_logprobs(z, tokens.cuda(), temperature=temperature)
+        _, want, want_h = oracle.rows(x, tokens, counted, temperature)
+        assert ((logp.detach().double().cpu() - want).abs() <= oracle.logp_bound(want)).all()
+        assert ((entropy.detach().double().cpu() - want_h).abs() <= 2 * oracle.logp_bound(want_h) + 2e-5).all()
+        # a small temperature multiplies the gradient: kept inside fp16's range
+        scale = min(1.0, temperature * 1e3)
+        grad, = torch.autograd.grad((logp, entropy), z, (scale * a.cuda(), scale * b.cuda()))
+        _check_far_grad(grad, x, tokens, temperature, scale * a.double(), scale * b.double())
+    # log p of the largest column is above -13 here: old_logp and the ratio are ordinary numbers
+    _, want, _ = oracle.rows(x, best, counted, temperature)
+    old, adv = want.float() + 0.1, torch.linspace(-1, 1, 8)
+    for entropy_coef in (0.0, 0.1):
+        out, grad = token_policy_loss_grad(x.cuda(), best.cuda(), old.cuda(), adv.cuda(), entropy_coef=entropy_coef,
+                                           temperature=temperature, grad_scale=scale)
+        loss, _, _, da, db = oracle.policy(x, best, old, adv, None, None, lo=0.8, hi=1.2, kl_coef=0.0, kind="k3",
+                                           entropy_coef=entropy_coef, temperature=temperature)
+        # logp and H within 3e-5, slopes of at most 2 |A| + 1
+        assert abs(out.loss.item() - loss) <= 1e-4
+        _check_far_grad(grad, x, best, temperature, scale * da, scale * db, slack=1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [37, 5000, 131075])
+@pytest.mark.parametrize("temperature,top", [(1.0, 2000.0), (1.0, 5e4), (1.0, -5e4), (0.5, -6e4), (1e-3, 30.0)])
+def test_large_logits(dtype, vocab, temperature, top):
+    """Logits far from zero are as exact as others: the shift of the exponents is one number for all of a row's columns."""
+    check_extreme(dtype, vocab, temperature, top)

@@ -200,7 +200,8 @@ struct Base {
   float inv, inv_lack;  // 1 / T as a sum
 };
 
-__device__ __forceinline__ float shift_of(float m, const Base& k) { return -m * k.hi; }
+// Rounded on its own: a product that the compiler fuses into the sum behind it is another shift than the columns' one.
+__device__ __forceinline__ float shift_of(float m, const Base& k) { return __fmul_rn(-m, k.hi); }
 
 // Rare, so by the accurate function: a chain of these with ex2.approx, which is low by 5e-8 on average, shows in sums.
 __device__ __forceinline__ void soft_raise(Soft& a, float m, const Base& k) {
@@ -292,7 +293,7 @@ __device__ __forceinline__ RowSoft row_soft(const Soft& a, const Base& k) {
   const bool normal = a.s > 1e-30f && a.s < 1e30f;
   const float e = normal ? static_cast<float>(static_cast<int>(bits >> 23) - 127) : 0.f;
   const float f = normal ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : a.s;
-  r.lns = e * kLn2;
+  r.lns = __fmul_rn(e, kLn2);
   const float td = a.t / a.s;
   r.mean = (td - off) / k.hi;
   const float rest = logf(f) + (fmaf(e, kLn2, -r.lns) + e * kLn2Lack);  // of the sums as they are
@@ -311,9 +312,9 @@ __device__ __forceinline__ float row_logp(const RowSoft& r, float z, const Base&
 // values: p_j = 2^((z_j - c) hi + 1 + f).
 __device__ __forceinline__ float2 row_shift(const RowSoft& r, const Base& k) {
   constexpr float kE = 1.44269504f, kELack = 1.92596299e-8f;  // log2(e) as a sum
-  const float l = r.lns * kE, l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.rest * kE;
+  const float l = __fmul_rn(r.lns, kE), l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.rest * kE;
   if (!(r.m > kLow)) return make_float2(r.m, -1.f - (l + l_lack));
-  const float p = r.m * k.hi, p_lack = fmaf(r.m, k.hi, -p);
+  const float p = __fmul_rn(r.m, k.hi), p_lack = fmaf(r.m, k.hi, -p);
   const float c = -(p + l), t = -c - p;  // c's own rounding by the two-sum
   const float lack = (p - (-c - t)) + (l - t) + p_lack + l_lack;
   // what hi lacks at the mean of z; the columns around it differ by less than a rounding
