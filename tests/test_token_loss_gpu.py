@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import token_oracle as oracle
-from test_token_loss import REFUSALS, extreme_rows, refuse, refuse_preference
+from test_token_loss import RANGES, REFUSALS, extreme_rows, refuse, refuse_preference
 from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
                                            token_policy_loss_grad)
 
@@ -461,4 +461,13 @@ def check_extreme(dtype, vocab, temperature, top):
 @pytest.mark.parametrize("temperature,top", [(1.0, 2000.0), (1.0, 5e4), (1.0, -5e4), (0.5, -6e4), (1e-3, 30.0)])
 def test_large_logits(dtype, vocab, temperature, top):
     """Logits far from zero are as exact as others: the shift of the exponents is one number for all of a row's columns."""
+    check_extreme(dtype, vocab, temperature, top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [37, 5000, 131075])
+@pytest.mark.parametrize("temperature,top", RANGES)
+def test_large_logits_over_temperature(dtype, vocab, temperature, top):
+    """Finite logits give finite results whatever their size over the temperature (the spacing of fp32 numbers as large
+    as |z| / T is far above one here, so the sums have to be of differences)."""
     check_extreme(dtype, vocab, temperature, top)

@@ -40,8 +40,8 @@ __device__ __forceinline__ Pair ex2(const Pair& x) {
   return Pair(ex2(lo), ex2(hi));
 }
 
-// Below this maximum c overflows: rows of lowest values subtract first. In the other rows a column below it counts as it:
-// its probability is zero, and that zero's products stay numbers.
+// In a row whose maximum is not far from zero (is_near) a column below this one counts as it: its probability is zero, and
+// that zero's products stay numbers.
 constexpr float kLow = -73786976294838206464.f;  // -2^66
 __device__ __forceinline__ float at_least_low(float z) {  // a NaN stays one
   float y;
@@ -185,7 +185,9 @@ __device__ __forceinline__ int64_t row_token(const TokenIndex& t, int64_t row, i
 
 // ---- running softmax ------------------------------------------------------------------------------------------------
 // The exponent of a column is d = z hi + c, one fused multiply-add, with c = -m hi for the largest z so far: any c near
-// -m hi serves as long as the sums and their use agree on it. `hi` is log2(e) / T rounded to a float; what it lacks (lo)
+// -m hi serves as long as the sums and their use agree on it, and c's rounding is at most 1/2 while |m| hi < 2^24. Beyond
+// that (logits of 1.2e7 at T = 1, of 12 at T = 1e-6; a row masked with -1e10 or the lowest value everywhere) the maximum is
+// subtracted first, d = (z - m) hi: exact up to z - m, where c would shift the exponents out of range. `hi` is log2(e) / T rounded to a float; what it lacks (lo)
 // shifts every exponent of a row the same way, an error that the sum over a sequence's rows would add up, so the end
 // corrects for it: d ln s / dk = sum p z.
 //
@@ -198,14 +200,23 @@ struct Soft {
 struct Base {
   float hi, lo;         // log2(e) / T as a sum
   float inv, inv_lack;  // 1 / T as a sum
+  float far;            // 2^24 / hi
 };
+
+__device__ __forceinline__ bool is_near(float m, const Base& k) { return fabsf(m) < k.far; }
 
 // Rounded on its own: a product that the compiler fuses into the sum behind it is another shift than the columns' one.
 __device__ __forceinline__ float shift_of(float m, const Base& k) { return __fmul_rn(-m, k.hi); }
 
+// The exponent of the maximum itself: what the rounding of c shifts all of its row's exponents by (exact).
+__device__ __forceinline__ float offset_of(float m, const Base& k) {
+  return is_near(m, k) ? fmaf(m, k.hi, shift_of(m, k)) : 0.f;
+}
+
 // Rare, so by the accurate function: a chain of these with ex2.approx, which is low by 5e-8 on average, shows in sums.
 __device__ __forceinline__ void soft_raise(Soft& a, float m, const Base& k) {
-  const float d = m > kLow && a.m > kLow ? shift_of(m, k) - shift_of(a.m, k) : (a.m - m) * k.hi;
+  const float d = is_near(m, k) && is_near(a.m, k) ? shift_of(m, k) - shift_of(a.m, k)
+                                                   : (a.m - m) * k.hi + (offset_of(m, k) - offset_of(a.m, k));
   const float f = expf(d * kLn2);
   a.t = f * fmaf(a.s, fmaxf(d, kFar), a.t);
   a.s *= f;
@@ -221,7 +232,7 @@ __device__ __forceinline__ void soft_absorb(Soft& a, const uint4* v, const Base&
 #pragma unroll
   for (int j = 1; j < kChunk; ++j) top = fmaxf(top, Elem<T>::top(v[j]));
   if (top > a.m) soft_raise(a, top, k);
-  if (a.m > kLow) {
+  if (is_near(a.m, k)) {
     const float c = shift_of(a.m, k);
     const Pair hi2(k.hi, k.hi), c2(c, c);
     Pair s[2] = {{0.f, 0.f}, {0.f, 0.f}}, t[2] = {{0.f, 0.f}, {0.f, 0.f}};
@@ -261,7 +272,7 @@ __device__ __forceinline__ void soft_absorb(Soft& a, const uint4* v, const Base&
 // One column.
 __device__ __forceinline__ void soft_absorb_one(Soft& a, float x, const Base& k) {
   if (x > a.m) soft_raise(a, x, k);
-  const float d = at_least_far(a.m > kLow ? fmaf(x, k.hi, shift_of(a.m, k)) : (x - a.m) * k.hi), e = ex2(d);
+  const float d = at_least_far(is_near(a.m, k) ? fmaf(x, k.hi, shift_of(a.m, k)) : (x - a.m) * k.hi), e = ex2(d);
   a.s += e;
   a.t = fmaf(e, d, a.t);
 }
@@ -279,7 +290,7 @@ __device__ __forceinline__ void soft_warp_reduce(Soft& a, const Base& k) {
 }
 
 // What a row's sums say: ln sum_j e^((z_j - m) / T) = lns + rest, where lns is a multiple of ln 2 and the rest below one, so
-// that a log-probability is rounded once. The rest has what the rounding of c and of hi has shifted (about 1e-6).
+// that a log-probability is rounded once. The rest has what the rounding of c and of hi has shifted (about 1e-6, at most 1/2).
 struct RowSoft {
   float m, lns, rest;
   float mean;  // of z - m under p
@@ -288,7 +299,7 @@ struct RowSoft {
 __device__ __forceinline__ RowSoft row_soft(const Soft& a, const Base& k) {
   RowSoft r;
   r.m = a.m;
-  const float off = a.m > kLow ? fmaf(a.m, k.hi, shift_of(a.m, k)) : 0.f;  // exact
+  const float off = offset_of(a.m, k);
   const uint32_t bits = __float_as_uint(a.s);
   const bool normal = a.s > 1e-30f && a.s < 1e30f;
   const float e = normal ? static_cast<float>(static_cast<int>(bits >> 23) - 127) : 0.f;
@@ -308,12 +319,12 @@ __device__ __forceinline__ float row_logp(const RowSoft& r, float z, const Base&
   const float back = y + r.lns;  // the rounding of y by the two-sum
   return y + (((x - back) + (back - y - r.lns)) - r.rest);
 }
-// What a gradient needs of a row: p_j = f 2^(z_j hi + c), f the rounding of c to a float; f < 0 marks a row of lowest
-// values: p_j = 2^((z_j - c) hi + 1 + f).
+// What a gradient needs of a row: p_j = f 2^(z_j hi + c), f the rounding of c to a float; f < 0 marks a row whose maximum is
+// far from zero: p_j = 2^((z_j - c) hi + 1 + f).
 __device__ __forceinline__ float2 row_shift(const RowSoft& r, const Base& k) {
   constexpr float kE = 1.44269504f, kELack = 1.92596299e-8f;  // log2(e) as a sum
   const float l = __fmul_rn(r.lns, kE), l_lack = fmaf(r.lns, kE, -l) + r.lns * kELack + r.rest * kE;
-  if (!(r.m > kLow)) return make_float2(r.m, -1.f - (l + l_lack));
+  if (!is_near(r.m, k)) return make_float2(r.m, -1.f - (l + l_lack));
   const float p = __fmul_rn(r.m, k.hi), p_lack = fmaf(r.m, k.hi, -p);
   const float c = -(p + l), t = -c - p;  // c's own rounding by the two-sum
   const float lack = (p - (-c - t)) + (l - t) + p_lack + l_lack;
@@ -681,6 +692,7 @@ Base base_of(double inv_temp) {
   b.lo = static_cast<float>(k - b.hi);
   b.inv = static_cast<float>(inv_temp);
   b.inv_lack = static_cast<float>(inv_temp - b.inv);
+  b.far = 16777216.f / b.hi;
   return b;
 }
 
