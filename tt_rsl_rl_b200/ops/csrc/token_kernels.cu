@@ -200,13 +200,11 @@ struct Soft {
 struct Base {
   float hi, lo;         // log2(e) / T as a sum
   float inv, inv_lack;  // 1 / T as a sum
-  float far;            // 2^24 / hi
 };
-
-__device__ __forceinline__ bool is_near(float m, const Base& k) { return fabsf(m) < k.far; }
 
 // Rounded on its own: a product that the compiler fuses into the sum behind it is another shift than the columns' one.
 __device__ __forceinline__ float shift_of(float m, const Base& k) { return __fmul_rn(-m, k.hi); }
+__device__ __forceinline__ bool is_near(float m, const Base& k) { return fabsf(shift_of(m, k)) < 16777216.f; }
 
 // The exponent of the maximum itself: what the rounding of c shifts all of its row's exponents by (exact).
 __device__ __forceinline__ float offset_of(float m, const Base& k) {
@@ -692,7 +690,6 @@ Base base_of(double inv_temp) {
   b.lo = static_cast<float>(k - b.hi);
   b.inv = static_cast<float>(inv_temp);
   b.inv_lack = static_cast<float>(inv_temp - b.inv);
-  b.far = 16777216.f / b.hi;
   return b;
 }
 
