@@ -471,3 +471,23 @@ def test_large_logits_over_temperature(dtype, vocab, temperature, top):
     """Finite logits give finite results whatever their size over the temperature (the spacing of fp32 numbers as large
     as |z| / T is far above one here, so the sums have to be of differences)."""
     check_extreme(dtype, vocab, temperature, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.5, 0.8, 1.0, 2.0])
+def test_token_at_the_lowest_value(dtype, temperature):
+    """A token whose column was masked with its type's lowest value: its log-probability is that value over T, or -inf
+    where this leaves fp32's range; never NaN."""
+    x, tokens, _, _ = _make((4,), 501, dtype, seed=12)
+    x[1, tokens[1]] = x[2, tokens[2]] = torch.finfo(dtype).min
+    logp, entropy = token_logprobs(x.cuda(), tokens.cuda(), temperature=temperature)
+    _, want, want_h = oracle.rows(x, tokens, torch.ones(4, dtype=torch.bool), temperature)
+    inf = want < -torch.finfo(torch.float32).max
+    assert inf.tolist() == [False, temperature < 1, temperature < 1, False]
+    assert torch.equal(logp.cpu()[inf], torch.full((int(inf.sum()),), float("-inf")))
+    assert ((logp.double().cpu() - want).abs() <= oracle.logp_bound(want))[~inf].all()
+    assert ((entropy.double().cpu() - want_h).abs() <= 2 * oracle.logp_bound(want_h) + 2e-5).all()
+    old = torch.where(want < -100, -5.0, want).float()  # the ratio of an excluded token is zero
+    out, grad = token_policy_loss_grad(x.cuda(), tokens.cuda(), old.cuda(), torch.ones(4, device="cuda"),
+                                       temperature=temperature)
+    assert out.loss.item() == pytest.approx(-0.5, abs=1e-4) and torch.isfinite(grad.float()).all()

@@ -312,8 +312,8 @@ __device__ __forceinline__ RowSoft row_soft(const Soft& a, const Base& k) {
 }
 __device__ __forceinline__ float row_logp(const RowSoft& r, float z, const Base& k) {
   const float d = z - r.m;
-  if (isinf(d)) return d - r.lns - r.rest;
-  const float x = fmaf(d, k.inv, d * k.inv_lack), y = x - r.lns;
+  const float x = isinf(d) ? d : fmaf(d, k.inv, d * k.inv_lack), y = x - r.lns;
+  if (isinf(x)) return y - r.rest;  // -inf, or the type's lowest value over a T below one; NaN where the sums are
   const float back = y + r.lns;  // the rounding of y by the two-sum
   return y + (((x - back) + (back - y - r.lns)) - r.rest);
 }
