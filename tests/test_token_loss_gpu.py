@@ -491,3 +491,16 @@ def test_token_at_the_lowest_value(dtype, temperature):
     out, grad = token_policy_loss_grad(x.cuda(), tokens.cuda(), old.cuda(), torch.ones(4, device="cuda"),
                                        temperature=temperature)
     assert out.loss.item() == pytest.approx(-0.5, abs=1e-4) and torch.isfinite(grad.float()).all()
+
+
+@pytest.mark.parametrize("shape", [(0,), (0, 5), (3, 0)])
+def test_backward_without_rows(shape):
+    z = torch.zeros(*shape, 9, device="cuda", requires_grad=True)
+    t, f = torch.zeros(shape, dtype=torch.long, device="cuda"), torch.zeros(shape, device="cuda")
+    losses = [token_policy_loss(z, t, f, f, ref_logp=f, kl_coef=0.1, entropy_coef=c).loss for c in (0.0, 0.1)]
+    losses.append(sum(x.sum() for x in token_logprobs(z, t)))
+    if shape != (3, 0):  # three sequences are no pairs
+        losses.append(preference_loss(z, t, offsets=None if len(shape) == 2 else t.new_zeros(1)).loss)
+    for loss in losses:
+        grad, = torch.autograd.grad(loss, z)
+        assert loss.item() == 0 and grad.shape == z.shape

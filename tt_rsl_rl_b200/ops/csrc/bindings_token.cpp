@@ -261,7 +261,7 @@ Tensor token_loss_backward(const Tensor& logits, const Tensor& tokens, const Opt
   const Logits l(logits);
   const c10::cuda::CUDAGuard guard(logits.device());
   const Index ix(l, tokens, mask);
-  const int64_t width = l.rows ? coef.numel() / l.rows : 1;
+  const int64_t width = coef.dim() == 2 ? coef.size(1) : 1;  // there may be no rows
   TORCH_CHECK_VALUE(ml.numel() == 2 * l.rows && coef.numel() == width * l.rows && (width == 1 || width == 2),
                     "token_loss_backward: statistics of other logits");
   Tensor grad = l.gradient();
