@@ -2,6 +2,7 @@
 
 import copy
 
+import numpy as np
 import pytest
 import torch
 
@@ -204,3 +205,29 @@ def test_refusals():
     assert CODES == torch.float8_e4m3fn
 
 
+
+
+def _norm_of(grads, max_norm=1.0):
+    """Norm that a clipped step returns, and the step's optimizer."""
+    params = [torch.nn.Parameter(torch.zeros_like(g, device="cuda")) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g.cuda()
+    opt = AdamW(params, max_grad_norm=max_norm, weight_decay=0.0, betas=(0.5, 0.5))
+    opt.step()
+    return opt.grad_norm.item(), opt
+
+
+@pytest.mark.parametrize("dtype,seed", [(torch.float32, 71), (torch.float32, 155), (torch.float32, 198),
+                                        (torch.bfloat16, 18), (torch.bfloat16, 224), (torch.bfloat16, 297)])
+def test_norm_of_growing_gradients(dtype, seed):
+    """Sums whose terms grow: every square is larger than the sum before it. The errors of its sixteen sums (2^-25 each) are
+    added up in fp32: 256 times 2^-49, so the sum is right to 2^-41 and the norm is the rounded one (half a step: 2^-24)
+    whatever the order. The seeds are some where error terms that assume the larger number first lead to a neighbour."""
+    rng = np.random.default_rng(seed)
+    chain = (1 + rng.random(16)) * 2.0 ** (np.arange(16) * rng.choice([0.5, 1.0, 2.0, 4.0]))
+    # runs of 2,048 elements in which each lane meets the sixteen numbers one after another
+    g = torch.tensor(chain, dtype=torch.float32).to(dtype).repeat_interleave(128).repeat(7104)
+    want = g.double().norm().item()
+    assert abs(_norm_of([g])[0] - want) <= want * (2.0 ** -24 + 2.0 ** -42)
+    back = g.flip(0)
+    assert abs(_norm_of([back])[0] - want) <= want * (2.0 ** -24 + 2.0 ** -42)

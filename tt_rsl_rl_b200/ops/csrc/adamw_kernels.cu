@@ -126,24 +126,28 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
 __device__ __forceinline__ float load1(const float* p) { return *p; }
 __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Sum of squares with its rounding errors: s + e is right to about 2^-45, so the norm in fp32 does not depend on the order
-// of the sum, at fp32 speed: summing in fp64 took 648 us for 335 M bf16 gradients, this 150 (4.5 TB/s). T. J. Dekker, "A
-// floating-point technique for extending the available precision" (1971): the error of s + x is x - ((s + x) - s) where s
-// is the larger; a sum of squares outgrows its terms.
+// Two sums of squares side by side, each with its rounding errors: s + e is right to about 2^-40 (hundreds of terms each), so
+// the norm in fp32 does not depend on the order of the sum, at fp32 speed: summing in fp64 took 648 us for 335 M bf16
+// gradients, this about 140 (4.8 TB/s). D. E. Knuth, "The Art of Computer Programming", volume 2: with t = s + x and
+// b = t - s, the error of t is (s - (t - b)) + (x - b), whichever of s and x is the larger (a gradient may outgrow all before
+// it).
 struct SquareSum {
-  float s = 0.f, e = 0.f;
+  Pair s = Pair(0.f, 0.f), e = Pair(0.f, 0.f);
   template <bool kExact>  // kExact: x * x fits fp32 (bf16 gradients)
-  __device__ __forceinline__ void add(float x) {
-    const float q = __fmul_rn(x, x);
-    if (!kExact) e = __fadd_rn(e, __fmaf_rn(x, x, -q));
-    const float t = __fadd_rn(s, q);
-    e = __fadd_rn(e, __fsub_rn(q, __fsub_rn(t, s)));
+  __device__ __forceinline__ void add(const Pair& x, const Pair& none) {
+    const Pair minus(-1.f, -1.f), q = fma2(x, x, none);  // a product of its own (AdamConsts::none)
+    if (!kExact) e = add2(e, fma2(x, x, mul2(q, minus)));
+    const Pair t = add2(s, q), b = fma2(s, minus, t);
+    e = add2(e, add2(fma2(fma2(b, minus, t), minus, s), fma2(b, minus, q)));
     s = t;
   }
   // s overflows (or holds a NaN): the errors are not numbers then, the sum is
   __device__ __forceinline__ double value() const {
-    const double big = static_cast<double>(s);
-    return isfinite(s) ? big + static_cast<double>(e) : big;
+    float big[2], small[2];
+    s.split(big[0], big[1]);
+    e.split(small[0], small[1]);
+    const double sum = static_cast<double>(big[0]) + static_cast<double>(big[1]);
+    return isfinite(sum) ? sum + (static_cast<double>(small[0]) + static_cast<double>(small[1])) : sum;
   }
 };
 
@@ -151,7 +155,7 @@ struct SquareSum {
 template <typename T, int K>
 __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_constant__ AdamTable<K> t,
                                                               const AdamHyper h, float* steps, AdamFactors* f,
-                                                              double* partial) {
+                                                              double* partial, float minus_zero) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
   __shared__ double smem[kWarps];
@@ -159,7 +163,8 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
   const int lane = threadIdx.x & 31;
   constexpr bool kExact = sizeof(T) == 2;
   constexpr int kBatch = kExact ? 4 : 2;  // units in flight: eight 8-byte or four 16-byte loads a lane
-  SquareSum sum[4];
+  SquareSum sum[2];
+  const Pair none(minus_zero, minus_zero);
   walk_units(t, [&](int ti, uint32_t first, uint32_t units) {
     const Entry& a = t.t[ti];
     const int64_t base = static_cast<int64_t>(first) * kAdamBlock;
@@ -172,18 +177,18 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 #pragma unroll
         for (int j = 0; j < 2 * kBatch; ++j) load4(g + at + j * 128 + lane * 4, x[j]);
 #pragma unroll
-        for (int i = 0; i < 8 * kBatch; ++i) sum[i & 3].template add<kExact>(x[i >> 2][i & 3]);
+        for (int i = 0; i < 4 * kBatch; ++i) sum[i & 1].template add<kExact>(Pair(x[i >> 1][2 * i & 2], x[i >> 1][2 * i & 2 | 1]), none);
       }
       for (; at + 128 <= left; at += 128) {
         float x[4];
         load4(g + at + lane * 4, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i].template add<kExact>(x[i]);
+        for (int i = 0; i < 2; ++i) sum[i].template add<kExact>(Pair(x[2 * i], x[2 * i + 1]), none);
       }
     }
-    for (at += lane; at < left; at += 32) sum[0].template add<kExact>(load1(g + at));
+    for (at += lane; at < left; at += 32) sum[0].template add<kExact>(Pair(load1(g + at), 0.f), none);
   });
-  double total = sum[0].value() + sum[1].value() + (sum[2].value() + sum[3].value());
+  double total = sum[0].value() + sum[1].value();
   total = block_sum64(total, smem);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
@@ -592,7 +597,7 @@ cudaError_t prepare(const AdamLaunch& a, AdamFactors* factors, Shared& sh, cudaS
     if (sh.max_norm > 0.0) {
       const unsigned grid = blocks_of(t.units, t.run, kNormBlocks);
       e = launch_pdl(adamw_norm_kernel<T, K>, dim3(grid), dim3(kThreads), 0, stream, t, a.h, a.steps, factors + first,
-                     sh.partial + sh.partials);
+                     sh.partial + sh.partials, -0.f);
       sh.partials += static_cast<int>(grid);
     } else {
       e = launch_pdl(adamw_prepare_kernel<K>, dim3(1), dim3(kThreads), 0, stream, t, a.h, a.steps, factors + first);
