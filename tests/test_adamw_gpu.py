@@ -231,3 +231,23 @@ def test_norm_of_growing_gradients(dtype, seed):
     assert abs(_norm_of([g])[0] - want) <= want * (2.0 ** -24 + 2.0 ** -42)
     back = g.flip(0)
     assert abs(_norm_of([back])[0] - want) <= want * (2.0 ** -24 + 2.0 ** -42)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-36, 1e-25, 1e-20, 1e-12, 1e18, 1e20, 1e25, 1e30])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_norm_beyond_the_range_of_squares(dtype, size, mixed):
+    """Gradients whose squares leave fp32's range: the norm is the 64-bit one rounded, and the step clips with it."""
+    gen = torch.Generator().manual_seed(3)
+    grads = [(torch.randn(n, generator=gen) * size).to(dtype) for n in (5, 3000, 70001, 256)]
+    if mixed:
+        grads[1][::2] = 1.0
+    want = torch.cat(grads).double().norm().item()
+    norm, opt = _norm_of(grads)
+    assert abs(norm - want) <= want * (2.0 ** -24 + 2.0 ** -42)
+    clip = min(1.0, 1.0 / (want + 1e-6))
+    for group in opt.param_groups:
+        for p, g in zip(group["params"], grads):
+            m = opt.state[p]["exp_avg"].double().cpu()
+            # clip, its product with g and the product with 0.5: half a step each, and subnormal numbers' spacing
+            assert ((m - 0.5 * clip * g.double()).abs() <= m.abs() * 2.0 ** -22 + 2.0 ** -148).all()

@@ -151,6 +151,10 @@ struct SquareSum {
   }
 };
 
+// Squares leave fp32's range above 1.8e19 (infinite) and lose digits below 4e-16. A block whose sum overflows, or is so small
+// that what its squares lost (2^-149 each) could show, sums its share again in fp64, whose range holds every square.
+constexpr double kLeastSum = 8.271806125530277e-25;  // 2^-80
+
 // Sum of the squares of every gradient, one partial per block; the last block also prepares the factors.
 template <typename T, int K>
 __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_constant__ AdamTable<K> t,
@@ -190,6 +194,20 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
   });
   double total = sum[0].value() + sum[1].value();
   total = block_sum64(total, smem);
+  if (!(total >= kLeastSum && isfinite(total))) {  // the same in every thread; gradients of zeros come here too
+    total = 0.0;
+    walk_units(t, [&](int ti, uint32_t first, uint32_t units) {
+      const Entry& a = t.t[ti];
+      const int64_t base = static_cast<int64_t>(first) * kAdamBlock;
+      const T* g = static_cast<const T*>(a.g) + base;
+      const int64_t left = min(a.n - base, static_cast<int64_t>(units) * kAdamBlock);
+      for (int64_t at = lane; at < left; at += 32) {
+        const double x = load1(g + at);
+        total = fma(x, x, total);
+      }
+    });
+    total = block_sum64(total, smem);
+  }
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
 
