@@ -251,3 +251,38 @@ def test_norm_beyond_the_range_of_squares(dtype, size, mixed):
             m = opt.state[p]["exp_avg"].double().cpu()
             # clip, its product with g and the product with 0.5: half a step each, and subnormal numbers' spacing
             assert ((m - 0.5 * clip * g.double()).abs() <= m.abs() * 2.0 ** -22 + 2.0 ** -148).all()
+
+
+def _quotients(m, v, eps):
+    """``-m' / (2 sqrt(v') + eps)`` as the step forms it, with m' = m / 2 and v' = 0.75 v, and as fp32 operations of
+    NumPy, each rounded correctly."""
+    p = torch.nn.Parameter(torch.zeros(len(m), device="cuda"))
+    p.grad = torch.zeros(len(m), device="cuda")
+    plan = AdamWPlan([p], [m.cuda()], [v.cuda()], torch.zeros(1, device="cuda"))
+    plan.step(lr=0.5, betas=(0.5, 0.75), eps=eps, weight_decay=0.0)  # lr / (1 - b1) = 1, 1 / sqrt(1 - b2) = 2
+    one = np.float32
+    with np.errstate(over="ignore"):
+        root = np.sqrt(v.numpy() * one(0.75))
+        return p.detach().cpu().numpy(), -(m.numpy() * one(0.5) / (root * one(2.0) + one(eps)))
+
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-20])
+def test_roots_and_quotients_are_rounded(eps):
+    """After the last Newton step the quotient is rounded from a value within 2^-21 of a step of the true one, the root
+    likewise: each is the rounded one but where the true one lies that close to the middle of two numbers (a chance of
+    about 2^-20 a number), and then it is the neighbour. A root that is off by a step moves the quotient by two at most."""
+    gen = torch.Generator().manual_seed(4)
+    n = 1 << 22
+    v = torch.exp((torch.rand(n, generator=gen) * 60 - 40) * 0.6931)  # 2^-40 to 2^20
+    m = torch.exp((torch.rand(n, generator=gen) * 60 - 30) * 0.6931) * (1 - 2 * (torch.rand(n, generator=gen) < 0.5).float())
+    got, want = _quotients(m, v, eps)
+    off = np.abs(got.view(np.int32).astype(np.int64) - want.view(np.int32).astype(np.int64))
+    assert off.max() <= 3 and (off > 0).mean() <= 1e-4
+
+
+def test_quotients_beyond_the_range_are_infinite():
+    m = torch.tensor([1e29, -1e29, 1e29, 1e25, 3e17, 0.0])
+    v = torch.tensor([1e-30, 1e-30, 1e20, 1e-38, 1e-38, 0.0])
+    got, want = _quotients(m, v, 1e-20)
+    assert not np.isnan(want).any() and np.isinf(want[:2]).all()
+    assert ((got == want) | (np.abs(got - want) <= np.abs(want) * 3 * 2.0 ** -23)).all()

@@ -255,10 +255,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
   return r;
 }
 
-// ---- correctly rounded roots and quotients, two at a time -----------------------------------------------------------------
+// ---- roots and quotients, two at a time -----------------------------------------------------------------------------------
 // P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor" (1990): Newton steps from an
-// approximation, then one step with the exact remainder. Right for 0 <= v < 1e30 and |a| < 1e30, 1e-20 <= d < 1e30 (below
-// about 1e-30 a result may be the neighbour of the rounded one); the functions of CUDA check for more and take one number.
+// approximation, then one step with the exact remainder, whose result is rounded from a value within about 2^-21 of a step of
+// the true one: the rounded one, but for one in a million that lies so near the middle of two numbers, where it may be the
+// neighbour (below about 1e-30 more often: the remainder is subnormal). For 0 <= v < 1e30 and |a| < 1e18, 1e-20 <= d < 1e30: a
+// quotient stays below 1e38 (an infinite one would leave a NaN as its remainder); the functions of CUDA check for more and
+// take one number.
 __device__ __forceinline__ Pair neg2(const Pair& a) { return mul2(a, Pair(-1.f, -1.f)); }
 
 __device__ __forceinline__ void sqrt2(const float (&v)[2], float (&r)[2]) {
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_co
         }
       }
       // the quick forms are for numbers: all lanes take the slow ones where one has to, and with a tiny eps
-      const bool quick = __all_sync(0xffffffffu, top[0] < 1e30f && top[1] < 1e30f) && c.eps >= 1e-20f;
+      const bool quick = __all_sync(0xffffffffu, top[0] < 1e18f && top[1] < 1e30f) && c.eps >= 1e-20f;
       const Pair unbias(f.unbias, f.unbias), eps(c.eps, c.eps), keep(f.decay, f.decay), rate(-f.step_size, -f.step_size);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
