@@ -207,3 +207,15 @@ def extreme_rows(dtype, top, vocab, seed=0):
 RANGES = [(1.0, -1e10), (1.0, 6e9), (1.0, -1e12), (1.0, 1e18), (1.0, -1e19), (1.0, -1e25), (1.0, 11629080.0),
           (1.0, -11629080.0), (1.0, 5e4), (1e-3, 3e6), (1e-3, 16000.0), (1e-3, -11629.08), (1e-6, 5000.0), (1e-6, 6e4),
           (1e-6, 11.62908), (1e-6, -11.62908), (1e6, 1e16), (0.5, -6e4)]
+
+
+def test_uint8_masks_select():
+    """Any value of a byte mask but zero counts a row once."""
+    logits, tokens, old, adv, ref, mask = _case((4, 7))
+    many = mask.to(torch.uint8) * 3
+    many[0, 0] = 255
+    mask[0, 0] = True
+    for a, b in ((token_policy_loss_grad(logits, tokens, old, adv, ref_logp=ref, mask=m, kl_coef=0.1, reduction="sum")
+                  for m in (many, mask)), (preference_loss_grad(logits, tokens, mask=m) for m in (many, mask))):
+        for x, y in zip((*a[0], a[1]), (*b[0], b[1])):
+            assert torch.equal(x, y)

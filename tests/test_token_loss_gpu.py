@@ -504,3 +504,11 @@ def test_backward_without_rows(shape):
     for loss in losses:
         grad, = torch.autograd.grad(loss, z)
         assert loss.item() == 0 and grad.shape == z.shape
+
+
+def test_uint8_masks_select():
+    x, tokens, old, adv, mask = _inputs(13)
+    for call in (lambda m: token_policy_loss_grad(x, tokens, old, adv, mask=m, reduction="sum"),
+                 lambda m: preference_loss_grad(x.view(6, 50, -1), tokens.view(6, 50), mask=m.view(6, 50))):
+        a, b = call(mask.to(torch.uint8) * 3), call(mask)
+        assert all(torch.equal(p, q) for p, q in zip((*a[0], a[1]), (*b[0], b[1])))

@@ -94,9 +94,11 @@ def _check_cpu(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | 
 
 # ---- log-probabilities ----------------------------------------------------------------------------------------------------
 def _row_weights(logits, tokens, mask) -> torch.Tensor:
-    """Weights of the rows; zero where the token lies outside the vocabulary."""
+    """Weights of the rows; zero where the token lies outside the vocabulary. Masks of bytes select (any value but zero)."""
     inside = (tokens >= 0) & (tokens < logits.shape[-1])
-    return inside.float() if mask is None else torch.where(inside, mask.float(), 0.0)
+    if mask is None:
+        return inside.float()
+    return torch.where(inside, mask if mask.dtype == torch.float32 else (mask != 0).float(), 0.0)
 
 
 def _logprobs_torch(logits, tokens, weights, temperature):
