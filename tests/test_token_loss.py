@@ -219,3 +219,24 @@ def test_uint8_masks_select():
                   for m in (many, mask)), (preference_loss_grad(logits, tokens, mask=m) for m in (many, mask))):
         for x, y in zip((*a[0], a[1]), (*b[0], b[1])):
             assert torch.equal(x, y)
+
+
+def only_logits_get_gradients(device):
+    """Every other input is a constant of the loss, floating masks and references too."""
+    logits, tokens, old, adv, ref, mask = (x.to(device) for x in _case((4, 7)))
+    z = logits.clone().requires_grad_()
+    rows = [x.clone().requires_grad_() for x in (old, adv, ref, mask.float())]
+    seq = torch.zeros(4, device=device, requires_grad=True)
+    token_policy_loss(z, tokens, rows[0], rows[1], ref_logp=rows[2], mask=rows[3], kl_coef=0.1, entropy_coef=0.1).loss.backward()
+    first, z.grad = z.grad, None
+    token_policy_loss(z, tokens, old, adv, ref_logp=ref, mask=mask.float(), kl_coef=0.1, entropy_coef=0.1).loss.backward()
+    assert torch.equal(first, z.grad)
+    preference_loss(z, tokens, seq, mask=rows[3], average=True).loss.backward()
+    assert seq.grad is None and all(x.grad is None for x in rows)
+    # without a gradient of the logits there is nothing to differentiate
+    assert not token_policy_loss(logits, tokens, rows[0], rows[1]).loss.requires_grad
+    assert not preference_loss(logits, tokens, seq).loss.requires_grad
+
+
+def test_only_logits_get_gradients():
+    only_logits_get_gradients("cpu")

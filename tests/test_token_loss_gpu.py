@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import token_oracle as oracle
-from test_token_loss import RANGES, REFUSALS, extreme_rows, refuse, refuse_preference
+from test_token_loss import RANGES, REFUSALS, extreme_rows, only_logits_get_gradients, refuse, refuse_preference
 from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
                                            token_policy_loss_grad)
 
@@ -512,3 +512,7 @@ def test_uint8_masks_select():
                  lambda m: preference_loss_grad(x.view(6, 50, -1), tokens.view(6, 50), mask=m.view(6, 50))):
         a, b = call(mask.to(torch.uint8) * 3), call(mask)
         assert all(torch.equal(p, q) for p, q in zip((*a[0], a[1]), (*b[0], b[1])))
+
+
+def test_only_logits_get_gradients():
+    only_logits_get_gradients("cuda")

@@ -6,7 +6,7 @@ vocabulary instead of a Gaussian. Logits are ``[rows, V]`` or ``[batch, rows, V]
 any row strides (``logits[:, :-1]`` is taken as it is) and contiguous columns; every other input is per row and float32.
 A row counts if its ``mask`` is not zero and its token lies in ``[0, V)``: the logits of no other row are read, its
 outputs and its gradient are zero. Columns at ``-inf`` have probability zero; a counted row without any finite column
-gives NaN, as the formulas do.
+gives NaN, as the formulas do. Gradients go to the logits alone: every other input is a constant.
 
 Each loss comes in two forms. ``*_loss`` is differentiable: it keeps a few numbers per row, and ``backward`` reads the
 logits once more. ``*_loss_grad`` returns the loss together with the gradient of the logits (in their type), without
@@ -92,6 +92,10 @@ def _check_cpu(logits: torch.Tensor, tokens: torch.Tensor, mask: torch.Tensor | 
         raise ValueError(f"temperature must lie in [1e-6, 1e6], got {temperature}")
 
 
+def _constant(x: torch.Tensor | None) -> torch.Tensor | None:
+    return None if x is None else x.detach()
+
+
 # ---- log-probabilities ----------------------------------------------------------------------------------------------------
 def _row_weights(logits, tokens, mask) -> torch.Tensor:
     """Weights of the rows; zero where the token lies outside the vocabulary. Masks of bytes select (any value but zero)."""
@@ -147,6 +151,7 @@ def _policy_settings(ref_logp, clip_param, clip_high, kl_coef, kl_estimator, ent
 
 
 def _policy_torch(logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind, entropy_coef, mean, temperature):
+    old, adv, ref, mask = map(_constant, (old, adv, ref, mask))
     w = _row_weights(logits, tokens, mask)
     counted = w != 0
     logp, entropy = _logprobs_torch(logits, tokens, w, temperature)
@@ -248,6 +253,7 @@ def _preference_settings(beta, label_smoothing, loss_type, average):
 
 
 def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind, average, temperature):
+    ref, mask = _constant(ref), _constant(mask)
     w = _row_weights(logits, tokens, mask)
     logp, _ = _logprobs_torch(logits, tokens, w, temperature)
     weighted = (w * logp).double()
