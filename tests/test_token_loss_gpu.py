@@ -516,3 +516,19 @@ def test_uint8_masks_select():
 
 def test_only_logits_get_gradients():
     only_logits_get_gradients("cuda")
+
+
+def test_forward_mode_is_refused():
+    """The kernels have no forward-mode derivative: a tangent of the logits is refused, not dropped."""
+    x, tokens, old, adv, mask = _inputs(14, 8, 100)
+    z = x.float()
+    forms = (lambda q: token_logprobs(q, tokens)[0], lambda q: token_policy_loss(q, tokens, old, adv).loss,
+             lambda q: token_policy_loss_grad(q, tokens, old, adv)[0].loss,
+             lambda q: preference_loss(q.view(2, 4, -1), tokens.view(2, 4)).loss,
+             lambda q: preference_loss_grad(q.view(2, 4, -1), tokens.view(2, 4))[0].loss)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(z, torch.ones_like(z))
+        for form in forms:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                form(dual)
+            form(z)

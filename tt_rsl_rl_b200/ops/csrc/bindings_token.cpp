@@ -52,6 +52,7 @@ struct Logits {
   rlb::TokenRows z;
   explicit Logits(const Tensor& x) : t(x), dtype(token_dtype(x)) {
     TORCH_CHECK_VALUE(x.is_cuda(), "logits must be a CUDA tensor");
+    TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined(), "the kernels have no forward-mode derivative by the logits");
     TORCH_CHECK_VALUE(x.dim() == 2 || x.dim() == 3, "logits must be [rows, V] or [batch, rows, V], got ", text(x.sizes()));
     vocab = x.size(-1);
     TORCH_CHECK_VALUE(vocab > 0, "logits need at least one column");

@@ -11,7 +11,7 @@ gives NaN, as the formulas do. Gradients go to the logits alone: every other inp
 Each loss comes in two forms. ``*_loss`` is differentiable: it keeps a few numbers per row, and ``backward`` reads the
 logits once more. ``*_loss_grad`` returns the loss together with the gradient of the logits (in their type), without
 autograd; it can be captured in a CUDA graph and is the faster one. On CPU tensors the same formulas run as PyTorch
-operations.
+operations. CUDA logits with a forward-mode tangent are refused.
 """
 
 from __future__ import annotations
