@@ -240,3 +240,28 @@ def only_logits_get_gradients(device):
 
 def test_only_logits_get_gradients():
     only_logits_get_gradients("cpu")
+
+
+def decided_pairs(device):
+    """A sequence that its policy excludes (log-probability -inf): as the rejected one its pair is decided, with a loss of
+    zero and no gradient; as the chosen one the loss is infinite. Without label smoothing nothing weighs the other side."""
+    logits, tokens, *_ = _case((4, 7), seed=5)
+    other = preference_loss_grad(logits[2:].to(device), tokens[2:].to(device), beta=0.2)
+    banned = logits.clone()
+    banned[1, 3, tokens[1, 3]] = float("-inf")
+    out, grad = preference_loss_grad(banned.to(device), tokens.to(device), beta=0.2)
+    assert out.rejected_rewards[0] == float("-inf")
+    # the mean over two pairs, one of them zero: half of the other's loss and gradient, rounded once more
+    assert out.loss.item() == pytest.approx(other[0].loss.item() / 2, rel=1e-6)
+    assert (grad[:2] == 0).all() and torch.allclose(grad[2:], other[1] / 2, rtol=1e-6, atol=0.0)
+    z = banned.clone().to(device).requires_grad_()
+    loss = preference_loss(z, tokens.to(device), beta=0.2).loss
+    loss.backward()
+    assert torch.equal(loss.detach(), out.loss) and torch.isfinite(z.grad).all()
+    banned[0, 2, tokens[0, 2]], banned[1] = float("-inf"), logits[1]
+    assert preference_loss(banned.to(device), tokens.to(device)).loss == float("inf")
+    assert preference_loss(banned.to(device), tokens.to(device), label_smoothing=0.1).loss == float("inf")
+
+
+def test_decided_pairs():
+    decided_pairs("cpu")

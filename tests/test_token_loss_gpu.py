@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import token_oracle as oracle
-from test_token_loss import RANGES, REFUSALS, extreme_rows, only_logits_get_gradients, refuse, refuse_preference
+from test_token_loss import (RANGES, REFUSALS, decided_pairs, extreme_rows, only_logits_get_gradients, refuse,
+                             refuse_preference)
 from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
                                            token_policy_loss_grad)
 
@@ -532,3 +533,7 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 form(dual)
             form(z)
+
+
+def test_decided_pairs():
+    decided_pairs("cuda")

@@ -1022,7 +1022,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
       const float h = static_cast<float>(rew[0] - rew[1]);
       float l, dh;  // loss of the pair and its derivative by h
       if (a.kind == kPrefSigmoid) {
-        l = (1.f - a.smoothing) * softplus_neg(h) + a.smoothing * softplus_neg(-h);
+        l = (1.f - a.smoothing) * softplus_neg(h);
+        if (a.smoothing != 0.f) l += a.smoothing * softplus_neg(-h);  // infinite for an infinite h
         dh = a.smoothing / (1.f + expf(-h)) - (1.f - a.smoothing) / (1.f + expf(h));
       } else if (a.kind == kPrefHinge) {
         l = isnan(h) ? h : fmaxf(1.f - h, 0.f);

@@ -283,7 +283,9 @@ def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind,
     h = rewards[0::2] - rewards[1::2]
     if kind == 0:
         log_sigmoid = torch.nn.functional.logsigmoid
-        losses = -(1.0 - smoothing) * log_sigmoid(h) - smoothing * log_sigmoid(-h)
+        losses = -(1.0 - smoothing) * log_sigmoid(h)
+        if smoothing:  # an infinite loss of the other side without a weight would leave a NaN
+            losses = losses - smoothing * log_sigmoid(-h)
     elif kind == 1:
         losses = torch.relu(1.0 - h)
     else:
