@@ -537,3 +537,30 @@ def test_forward_mode_is_refused():
 
 def test_decided_pairs():
     decided_pairs("cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.0, False), ("sigmoid", 0.1, False), ("sigmoid", 0.3, True),
+                                                    ("hinge", 0.0, False), ("hinge", 0.0, True), ("ipo", 0.0, False),
+                                                    ("ipo", 0.0, True)])
+def test_preference_losses(dtype, kind, smoothing, average):
+    """Each loss's value in all of its forms, for pairs on both sides of its border."""
+    x, tokens, mask, _ = _make((8, 9), 301, dtype, seed=15)
+    bounds = [(9 * i, 9 * i + 9) for i in range(8)]
+    lps = oracle.preference(x, tokens, None, bounds, mask, beta=0.2, average=average)[1]
+    h = torch.tensor([-6.0, -0.4, 0.7, 9.0])  # differences of rewards
+    ref = lps.float()
+    ref[0::2] -= h / 0.2
+    loss = oracle.preference(x, tokens, ref, bounds, mask, beta=0.2, smoothing=smoothing, kind=kind, average=average)[0]
+    kwargs = dict(mask=mask.cuda(), beta=0.2, label_smoothing=smoothing, loss_type=kind, average=average)
+    # a sequence's log-probability is off by at most 9 bounds of a row's (|logp| < 25: 1.6e-5 each), h by twice beta times
+    # that (6e-5) and its own rounding in fp32 (2^-21); the slopes by h are at most 1 (sigmoid, hinge) and
+    # 2 (|h| + 0.5) / beta^2 = 475 (ipo), and the value is rounded
+    tol = (6e-5 + 2.0 ** -21) * (475 if kind == "ipo" else 1) + 2.0 ** -22 * abs(loss)
+    forms = [preference_loss_grad(x.cuda(), tokens.cuda(), ref.cuda(), **kwargs)[0].loss,
+             preference_loss(x.cuda(), tokens.cuda(), ref.cuda(), **kwargs).loss,
+             preference_loss(x.cuda().requires_grad_(), tokens.cuda(), ref.cuda(), **kwargs).loss,
+             preference_loss(x.cuda().flatten(0, 1), tokens.cuda().flatten(), ref.cuda(),
+                             offsets=torch.arange(0, 73, 9).cuda(), **(kwargs | {"mask": mask.cuda().flatten()})).loss]
+    for got in forms:
+        assert abs(got.item() - loss) <= tol
