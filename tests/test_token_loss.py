@@ -265,3 +265,15 @@ def decided_pairs(device):
 
 def test_decided_pairs():
     decided_pairs("cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("temperature,top", RANGES)
+def test_large_logits_over_temperature(dtype, temperature, top):
+    if dtype == torch.float16 and abs(top) > 6e4:
+        return
+    x, tokens = extreme_rows(dtype, top, 503)
+    logp, entropy = token_logprobs(x, tokens, temperature=temperature)
+    _, want, want_h = oracle.rows(x, tokens, torch.ones(8, dtype=torch.bool), temperature)
+    assert ((logp.double() - want).abs() <= oracle.logp_bound(want)).all()
+    assert ((entropy.double() - want_h).abs() <= 2 * oracle.logp_bound(want_h) + 2e-5).all()

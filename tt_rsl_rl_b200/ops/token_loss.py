@@ -108,13 +108,14 @@ def _row_weights(logits, tokens, mask) -> torch.Tensor:
 def _logprobs_torch(logits, tokens, weights, temperature):
     counted = weights != 0
     # rows that do not count take part with zeros, so that nothing of them (NaN included) reaches a gradient
-    z = torch.where(counted[..., None], logits.float(), 0.0) / temperature
+    # in 64 bits: a quotient by a small temperature would round the columns' differences away
+    z = torch.where(counted[..., None], logits.double(), 0.0) / temperature
     log_p = torch.log_softmax(z, -1)
     tok = tokens.long().clamp(0, logits.shape[-1] - 1)
     logp = log_p.gather(-1, tok[..., None])[..., 0]
     dead = log_p == float("-inf")
     entropy = -(log_p.exp() * log_p.masked_fill(dead, 0.0)).sum(-1)
-    return torch.where(counted, logp, 0.0), torch.where(counted, entropy, 0.0)
+    return torch.where(counted, logp, 0.0).float(), torch.where(counted, entropy, 0.0).float()
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Tensor | None = None,
