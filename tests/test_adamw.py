@@ -339,3 +339,29 @@ def test_refusals():
 def test_names_resolve():
     assert resolve_optimizer("adamw_fused") is AdamW and resolve_optimizer("AdamW_8bit") is AdamW8bit
     assert resolve_optimizer("adamw") is torch.optim.AdamW
+
+
+def test_hooks_of_loading():
+    """A hook before loading changes what is loaded, one behind it what was; types stay those of the states."""
+    p, q = (torch.ones(300, dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    first, second = AdamW([p]), AdamW([q])
+    p.grad = torch.full_like(p, 0.5)
+    first.step()
+
+    def before(_, state):
+        state = copy.deepcopy(state)
+        state["state"][0]["exp_avg"].mul_(2.0)
+        return state
+
+    second.register_load_state_dict_pre_hook(before)
+    second.register_load_state_dict_post_hook(lambda opt: opt.state[q]["exp_avg_sq"].zero_())
+    second.load_state_dict(first.state_dict())
+    assert second.state[q]["exp_avg"].dtype == torch.float32
+    assert torch.equal(second.state[q]["exp_avg"], 2 * first.state[p]["exp_avg"])
+    assert (second.state[q]["exp_avg_sq"] == 0).all() and (first.state[p]["exp_avg_sq"] > 0).all()
+    refused = torch.optim.AdamW([p], amsgrad=True)
+    refused.register_load_state_dict_pre_hook(lambda *_: None)
+    third = AdamW([q])
+    third.register_load_state_dict_pre_hook(lambda _, state: {**state, "param_groups": [
+        {**g, "amsgrad": False} for g in state["param_groups"]]})
+    third.load_state_dict({"state": {}, "param_groups": refused.state_dict()["param_groups"]})

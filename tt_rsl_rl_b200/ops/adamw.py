@@ -278,19 +278,33 @@ class AdamW(torch.optim.Optimizer):
         self._plans = None
 
     def load_state_dict(self, state_dict) -> None:
-        """The base class casts states to the parameter's type; codes, scales and float32 moments keep theirs here."""
-        for group in state_dict["param_groups"]:
-            if group.get("amsgrad"):
-                raise ValueError("AdamW: the loaded state is of an update with amsgrad, which this one has not")
-            if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0.0) != 0.0:
-                raise ValueError("AdamW: the loaded state is of an update whose weight decay is not decoupled")
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        super().load_state_dict(state_dict)
-        own = [p for group in self.param_groups for p in group["params"]]
-        for index, p in zip(saved, own):
-            for key, value in state_dict["state"].get(index, {}).items():
-                if isinstance(value, torch.Tensor):
-                    self.state[p][key] = value.detach().to(device=p.device, copy=True)
+        """The base class casts states to the parameter's type; codes, scales and float32 moments keep theirs here: as the
+        last hook before loading leaves them, and before the first one behind it."""
+        loaded = {}
+
+        def check(_, state):
+            for group in state["param_groups"]:
+                if group.get("amsgrad"):
+                    raise ValueError("AdamW: the loaded state is of an update with amsgrad, which this one has not")
+                if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0.0) != 0.0:
+                    raise ValueError("AdamW: the loaded state is of an update whose weight decay is not decoupled")
+            loaded.update(state)
+
+        def keep_types(_):
+            saved = [i for group in loaded["param_groups"] for i in group["params"]]
+            own = [p for group in self.param_groups for p in group["params"]]
+            for index, p in zip(saved, own):
+                for key, value in loaded["state"].get(index, {}).items():
+                    if isinstance(value, torch.Tensor):
+                        self.state[p][key] = value.detach().to(device=p.device, copy=True)
+
+        hooks = (self.register_load_state_dict_pre_hook(check),
+                 self.register_load_state_dict_post_hook(keep_types, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
         self._plans = None
 
     def _state_of(self, p: torch.Tensor) -> dict:
