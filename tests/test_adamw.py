@@ -365,3 +365,18 @@ def test_hooks_of_loading():
     third.register_load_state_dict_pre_hook(lambda _, state: {**state, "param_groups": [
         {**g, "amsgrad": False} for g in state["param_groups"]]})
     third.load_state_dict({"state": {}, "param_groups": refused.state_dict()["param_groups"]})
+
+
+def test_codes_without_scales_are_refused():
+    """8-bit codes mean nothing without their scales: they are not taken as zero."""
+    p = torch.ones(300).requires_grad_()
+    p.grad = torch.ones(300)
+    first = AdamW8bit([p])
+    first.step()
+    for key in ("exp_avg_scale", "exp_avg_sq_scale"):
+        state = copy.deepcopy(first.state_dict())
+        del state["state"][0][key]
+        second = AdamW8bit([p])
+        second.load_state_dict(state)
+        with pytest.raises(ValueError, match=key):
+            second.step()

@@ -320,6 +320,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"the loaded {key} is {x.dtype}: it does not belong to {self.state_bits}-bit states")
             if x.shape != p.shape:
                 raise ValueError(f"the loaded {key} has the shape {tuple(x.shape)}, its parameter {tuple(p.shape)}")
+            if self.state_bits == 8 and state.get(f"{key}_scale") is None:
+                raise ValueError(f"the loaded {key} has no {key}_scale: 8-bit codes mean nothing without their scales")
             if self.state_bits == 8 and not _same_order(x, p):
                 raise ValueError(f"the loaded {key} has strides {x.stride()}, its parameter {p.stride()}: the scales of "
                                  "8-bit states follow the order in memory")
