@@ -653,7 +653,6 @@ void rlb_register_token(pybind11::module& m) {
                                        PreferenceSettings{beta, smoothing, kind, average, temperature});
         });
   m.def("preference_loss", &preference_loss);
-  m.attr("adamw_block") = rlb::kAdamBlock;
   pybind11::class_<AdamWPlan>(m, "AdamWPlan")
       .def(pybind11::init<std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, Tensor, std::vector<Tensor>,
                           std::vector<Tensor>, std::vector<Tensor>, int64_t>());
