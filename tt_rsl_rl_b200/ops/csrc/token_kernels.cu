@@ -213,8 +213,10 @@ __device__ __forceinline__ float offset_of(float m, const Base& k) {
 
 // Rare, so by the accurate function: a chain of these with ex2.approx, which is low by 5e-8 on average, shows in sums.
 __device__ __forceinline__ void soft_raise(Soft& a, float m, const Base& k) {
-  const float d = is_near(m, k) && is_near(a.m, k) ? shift_of(m, k) - shift_of(a.m, k)
-                                                   : (a.m - m) * k.hi + (offset_of(m, k) - offset_of(a.m, k));
+  float d = shift_of(m, k) - shift_of(a.m, k);
+  if (__builtin_expect(!(is_near(m, k) && is_near(a.m, k)), 0)) {
+    d = (a.m - m) * k.hi + (offset_of(m, k) - offset_of(a.m, k));
+  }
   const float f = expf(d * kLn2);
   a.t = f * fmaf(a.s, fmaxf(d, kFar), a.t);
   a.s *= f;
@@ -230,7 +232,7 @@ __device__ __forceinline__ void soft_absorb(Soft& a, const uint4* v, const Base&
 #pragma unroll
   for (int j = 1; j < kChunk; ++j) top = fmaxf(top, Elem<T>::top(v[j]));
   if (top > a.m) soft_raise(a, top, k);
-  if (is_near(a.m, k)) {
+  if (__builtin_expect(is_near(a.m, k), 1)) {
     const float c = shift_of(a.m, k);
     const Pair hi2(k.hi, k.hi), c2(c, c);
     Pair s[2] = {{0.f, 0.f}, {0.f, 0.f}}, t[2] = {{0.f, 0.f}, {0.f, 0.f}};
