@@ -206,7 +206,7 @@ def extreme_rows(dtype, top, vocab, seed=0):
 # 2^24 / log2(e) = 11,629,080 too (the largest fp32 logits there are a unit of the exponent apart).
 RANGES = [(1.0, -1e10), (1.0, 6e9), (1.0, -1e12), (1.0, 1e18), (1.0, -1e19), (1.0, -1e25), (1.0, 11629080.0),
           (1.0, -11629080.0), (1.0, 5e4), (1e-3, 3e6), (1e-3, 16000.0), (1e-3, -11629.08), (1e-6, 5000.0), (1e-6, 6e4),
-          (1e-6, 11.62908), (1e-6, -11.62908), (1e6, 1e16), (0.5, -6e4)]
+          (1e-6, 11.62908), (1e-6, -11.62908), (1e6, 1e16), (1e6, -1.162908e13), (1.0, 3e38), (1.0, -3e38), (0.5, -6e4)]
 
 
 def test_uint8_masks_select():
