@@ -2,6 +2,7 @@
 
 import copy
 
+import numpy as np
 import pytest
 import torch
 
@@ -380,3 +381,17 @@ def test_codes_without_scales_are_refused():
         second.load_state_dict(state)
         with pytest.raises(ValueError, match=key):
             second.step()
+
+
+def test_roots_are_rounded():
+    """Roots and quotients are correctly rounded, as the kernels' roots are (those of PyTorch's CPU operations may be a step
+    off)."""
+    gen = torch.Generator().manual_seed(6)
+    m, v = torch.randn(1 << 20, generator=gen), torch.rand(1 << 20, generator=gen) * 10
+    p = torch.zeros(1 << 20)
+    p.grad = torch.zeros(1 << 20)
+    one = np.float32
+    want = -(m.numpy() * one(0.5) / (np.sqrt(v.numpy() * one(0.75)) * one(2.0) + one(1e-8)))
+    # lr / (1 - b1) = 1, 1 / sqrt(1 - b2) = 2
+    AdamWPlan([p], [m], [v], torch.zeros(1)).step(lr=0.5, betas=(0.5, 0.75), eps=1e-8, weight_decay=0.0)
+    assert (p.numpy() == want).all()

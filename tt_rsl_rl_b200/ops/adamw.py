@@ -222,7 +222,7 @@ def _step_torch(plans, settings, max_grad_norm):
                 v1 = v0 * b2 + g * g * (1 - b2)
                 t = float(steps[i])
                 step_size, unbias, keep = torch.tensor([lr / (1 - b1 ** t), (1 - b2 ** t) ** -0.5, 1 - lr * decay])
-                root = v1.sqrt()
+                root = v1.double().sqrt().float()  # rounded correctly, which an fp32 root here may not be
                 x = x * keep - step_size * (m1 / (root * unbias + eps))
                 if low:
                     bits = x.view(torch.int32)
