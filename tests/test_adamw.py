@@ -395,3 +395,26 @@ def test_roots_are_rounded():
     # lr / (1 - b1) = 1, 1 / sqrt(1 - b2) = 2
     AdamWPlan([p], [m], [v], torch.zeros(1)).step(lr=0.5, betas=(0.5, 0.75), eps=1e-8, weight_decay=0.0)
     assert (p.numpy() == want).all()
+
+
+def spikes(device):
+    """A finite gradient whose square leaves fp32's range makes its block's second moment infinite: the block's weights
+    stay where they are, the other blocks do not see it."""
+    ends = []
+    for spike in (1.0, 1e25):
+        p = torch.ones(600, device=device).requires_grad_()
+        opt = AdamW8bit([p], weight_decay=0.0)
+        for step in range(3):
+            p.grad = torch.linspace(-1, 1, 600, device=device)
+            p.grad[3] = spike if step == 0 else 1.0
+            opt.step()
+            if step == 0:
+                held = p.detach()[:256].clone()
+        assert opt.state[p]["exp_avg_sq_scale"].isinf().tolist() == [spike > 1, False, False]
+        ends.append((held, p.detach().clone()))
+    assert torch.equal(ends[0][1][256:], ends[1][1][256:])
+    assert torch.equal(ends[1][1][:256], ends[1][0]) and torch.isfinite(ends[1][0]).all()
+
+
+def test_spikes():
+    spikes("cpu")

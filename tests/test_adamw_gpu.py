@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_adamw import (HYPER, SHAPES, check_step, make_plan, refuse_plans, resume, rounding_statistics, whole,
+from test_adamw import (HYPER, SHAPES, check_step, make_plan, refuse_plans, resume, rounding_statistics, spikes, whole,
                         zeros_written)
 from tt_rsl_rl_b200.ops.adamw import CODES, AdamW, AdamW8bit, AdamWPlan
 
@@ -286,3 +286,7 @@ def test_quotients_beyond_the_range_are_infinite():
     got, want = _quotients(m, v, 1e-20)
     assert not np.isnan(want).any() and np.isinf(want[:2]).all()
     assert ((got == want) | (np.abs(got - want) <= np.abs(want) * 3 * 2.0 ** -23)).all()
+
+
+def test_spikes():
+    spikes("cuda")

@@ -523,6 +523,9 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_co
             for (int i = 0; i < 2; ++i) r[i] = __fsqrt_rn(v[i]);
             x = Pair(__fdiv_rn(m[0], __fadd_rn(__fmul_rn(r[0], f.unbias), c.eps)),
                      __fdiv_rn(m[1], __fadd_rn(__fmul_rn(r[1], f.unbias), c.eps)));
+            if (kBits8) {  // as the codes take it; a NaN stays one in its block's scale
+              for (int i = 0; i < 2; ++i) r[i] = fminf(r[i], 3e38f);
+            }
           }
           add2(fma2(Pair(q[j].p[e], q[j].p[e + 1]), keep, none), fma2(rate, x, none)).split(q[j].p[e], q[j].p[e + 1]);
           if (kBits8) q[j].v[e] = r[0], q[j].v[e + 1] = r[1];
@@ -538,7 +541,8 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_co
         // blocks below 1e-30 are held as zero, so the scale's inverse stays finite
         const bool m_on = !(m_top < 1e-30f), r_on = !(r_top < 1e-30f);
         const float mi = m_on ? __fmul_rn(__frcp_rn(m_top), 448.f) : 0.f;
-        const float ri = r_on ? __fmul_rn(__frcp_rn(r_top), 448.f) : 0.f;
+        // a root beyond fp32 leaves an infinite scale: no code is zero or a NaN then, so that all of the block stay infinite
+        const float ri = r_on ? fmaxf(__fmul_rn(__frcp_rn(r_top), 448.f), 1e-38f) : 0.f;
         if (lane == 0) {
           a.m_scale[u] = m_on ? __fmul_rn(m_top, 1.f / 448.f) : 0.f;
           a.v_scale[u] = r_on ? __fmul_rn(r_top, 1.f / 448.f) : 0.f;
