@@ -11,9 +11,12 @@ and of the *root* of the second, whose range a code covers better. One step move
 distance between two codes, so a code is rounded up or down at random with the probabilities that make the stored first
 and second moments right on average (Philox4x32-10, keyed by ``seed``; counted by element, tensor and step, so equal
 seeds give equal steps on every rank). A root never rounds down to zero, which would leave ``m / eps`` as a step. Blocks
-whose largest moment is below 1e-30 are stored as zero; a NaN or infinity makes its block's scale NaN or infinite.
+whose largest moment is below 1e-30 are stored as zero; a NaN or infinity makes its block's scale NaN or infinite. A finite
+gradient whose square is beyond float32 (1.8e19 and more, unless it is clipped) makes its block's second moment infinite, so
+the block's weights stay where they are.
 
-The learning rate may be a tensor on the device; a captured step (after one eager one) reads it at every replay, and
+The gradients' norm is right to float32's rounding over their whole range, whatever the order and split of the tensors. The
+learning rate may be a tensor on the device; a captured step (after one eager one) reads it at every replay, and
 advances the step counts, which are on the device too. On CPU tensors the same arithmetic runs as PyTorch operations.
 """
 

@@ -128,12 +128,12 @@ __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat
 
 // Two sums of squares side by side, each with its rounding errors: s + e is right to about 2^-40 (hundreds of terms each), so
 // the norm in fp32 does not depend on the order of the sum, at fp32 speed: summing in fp64 took 648 us for 335 M bf16
-// gradients, this about 140 (4.8 TB/s). D. E. Knuth, "The Art of Computer Programming", volume 2: with t = s + x and
+// gradients, this 139 for one tensor, 152 for 194 (4.4 TB/s). D. E. Knuth, "The Art of Computer Programming", volume 2: with t = s + x and
 // b = t - s, the error of t is (s - (t - b)) + (x - b), whichever of s and x is the larger (a gradient may outgrow all before
 // it).
 struct SquareSum {
   Pair s = Pair(0.f, 0.f), e = Pair(0.f, 0.f);
-  template <bool kExact>  // kExact: x * x fits fp32 (bf16 gradients)
+  template <bool kExact>  // kExact: x * x fits fp32 where it is in range (bf16 gradients)
   __device__ __forceinline__ void add(const Pair& x, const Pair& none) {
     const Pair minus(-1.f, -1.f), q = fma2(x, x, none);  // a product of its own (AdamConsts::none)
     if (!kExact) e = add2(e, fma2(x, x, mul2(q, minus)));
@@ -181,7 +181,9 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 #pragma unroll
         for (int j = 0; j < 2 * kBatch; ++j) load4(g + at + j * 128 + lane * 4, x[j]);
 #pragma unroll
-        for (int i = 0; i < 4 * kBatch; ++i) sum[i & 1].template add<kExact>(Pair(x[i >> 1][2 * i & 2], x[i >> 1][2 * i & 2 | 1]), none);
+        for (int i = 0; i < 4 * kBatch; ++i) {
+          sum[i & 1].template add<kExact>(Pair(x[i >> 1][2 * i & 2], x[i >> 1][2 * i & 2 | 1]), none);
+        }
       }
       for (; at + 128 <= left; at += 128) {
         float x[4];
@@ -259,7 +261,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN wins
 // P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor" (1990): Newton steps from an
 // approximation, then one step with the exact remainder, whose result is rounded from a value within about 2^-21 of a step of
 // the true one: the rounded one, but for one in a million that lies so near the middle of two numbers, where it may be the
-// neighbour (below about 1e-30 more often: the remainder is subnormal). For 0 <= v < 1e30 and |a| < 1e18, 1e-20 <= d < 1e30: a
+// neighbour (none of 67 million pairs; below about 1e-30 more often: the remainder is subnormal). For 0 <= v < 1e30 and |a| < 1e18, 1e-20 <= d < 1e30: a
 // quotient stays below 1e38 (an infinite one would leave a NaN as its remainder); the functions of CUDA check for more and
 // take one number.
 __device__ __forceinline__ Pair neg2(const Pair& a) { return mul2(a, Pair(-1.f, -1.f)); }
@@ -455,7 +457,7 @@ struct Quad {
 // A warp takes units of 256 elements: lane l elements [4 l, 4 l + 4) and [128 + 4 l, ...), so every access of the warp is
 // contiguous. The unit is also the block of a scale, whose maximum is a warp reduction. With 32-bit states the step is
 // bound by memory; with 8-bit states by its instructions, about 110 an element (random numbers, both roundings, root and
-// quotient): 335 M bf16 weights in 1,501 us, 2.1 times the bytes' time, with 70 % of the issue slots used. Codes taken and
+// quotient): 335 M bf16 weights in 1,497 us, 2.1 times the bytes' time, with 70 % of the issue slots used. Codes taken and
 // packed by shifts and products instead of conversions, and pairs, brought it there from 2,832.
 template <typename T, bool kBits8, int K>
 __global__ void __launch_bounds__(kThreads, 3) adamw_step_kernel(const __grid_constant__ AdamTable<K> t,

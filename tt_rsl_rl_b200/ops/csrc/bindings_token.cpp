@@ -83,7 +83,8 @@ struct Logits {
            same(t.stride(-2), grad.stride(-2)) && (t.dim() == 2 || same(t.stride(0), grad.stride(0)));
   }
   // Where rows start at different places within 16 bytes, the gradient takes the logits' strides (if that costs at most
-  // a quarter more memory), so that both can be accessed 16 bytes at a time.
+  // a quarter more memory), so that both can be accessed 16 bytes at a time. A whole number of 16 bytes in rows that are
+  // padded to another pitch (a slice of a padded vocabulary) is left contiguous: its rows take the slower kernels.
   Tensor gradient() const {
     const int64_t size = t.element_size();
     bool wide = (vocab * size) % 16 == 0;

@@ -22,6 +22,8 @@ constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f, kLn2Lack = -1.90465429995776e-9f;  // ln 2 as a sum
 constexpr float kFar = -1e30f;  // exponent of a column of probability zero: its product with that zero stays a number
 
+// One instruction, within 2^-22 of 2^x; results below 2^-126 are zero. What is summed over columns is no more exact than that;
+// what is done once a row uses the accurate functions.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -187,9 +189,9 @@ __device__ __forceinline__ int64_t row_token(const TokenIndex& t, int64_t row, i
 // The exponent of a column is d = z hi + c, one fused multiply-add, with c = -m hi for the largest z so far: any c near
 // -m hi serves as long as the sums and their use agree on it, and c's rounding is at most 1/2 while |m| hi < 2^24. Beyond
 // that (logits of 1.2e7 at T = 1, of 12 at T = 1e-6; a row masked with -1e10 or the lowest value everywhere) the maximum is
-// subtracted first, d = (z - m) hi: exact up to z - m, where c would shift the exponents out of range. `hi` is log2(e) / T rounded to a float; what it lacks (lo)
-// shifts every exponent of a row the same way, an error that the sum over a sequence's rows would add up, so the end
-// corrects for it: d ln s / dk = sum p z.
+// subtracted first, d = (z - m) hi: c would shift the exponents out of range there. `hi` is log2(e) / T rounded to a float;
+// what it lacks (lo) shifts every exponent of a row the same way, an error that the sum over a sequence's rows would add up,
+// so the end corrects for it: d ln s / dk = sum p z.
 //
 // m: maximum so far (starts at the lowest finite value, so rows and columns at that value or at -inf stay defined),
 // s: sum of 2^d, t: sum of 2^d d.
@@ -290,7 +292,8 @@ __device__ __forceinline__ void soft_warp_reduce(Soft& a, const Base& k) {
 }
 
 // What a row's sums say: ln sum_j e^((z_j - m) / T) = lns + rest, where lns is a multiple of ln 2 and the rest below one, so
-// that a log-probability is rounded once. The rest has what the rounding of c and of hi has shifted (about 1e-6, at most 1/2).
+// that a log-probability is rounded once. The rest has what the rounding of c and of hi has shifted (about 1e-6 for ordinary
+// logits, at most 1/2).
 struct RowSoft {
   float m, lns, rest;
   float mean;  // of z - m under p
@@ -507,7 +510,7 @@ __device__ __forceinline__ void zero_row(T* out, int64_t vocab, int rank, int ra
 // ---- row statistics -----------------------------------------------------------------------------------------------------
 // A CTA per row, or a cluster of them where rows are few: each CTA a share of the row's vectors, whose sums meet in every
 // CTA's shared memory. Bound by memory for fp32 (737 MB in 116 us, 97 % of the copy rate); for bf16 by the instructions of
-// a column too (one ex2 of the special-function unit, about seven others): 268 MB in 60 us, 2.1 GB in 316 us (95 %).
+// a column too (7.9 of them, one the ex2 of the special-function unit): 268 MB in 60 us, 2.1 GB in 316 us (95 %).
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 4) token_stats_kernel(const TokenStatsArgs a, const PolicyTerms q,
                                                                       bool policy, const Base k) {
@@ -582,7 +585,7 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double* smem) {
 
 // A CTA or cluster per row as above, which turns to the row a second time for its gradient as soon as its sums are known:
 // the rows in work fit L2 (row_launch), and loads that say which read is the last keep them there. Measured at 8,192 rows
-// of 131,072 bf16 columns (a tenth masked): 886 us, where statistics and gradient as two kernels take 316 + 663; memory
+// of 131,072 bf16 columns (a tenth masked): 888 us, where statistics and gradient as two kernels take 316 + 663; memory
 // traffic is 1.15 times one read and one write, so most second reads hit. What remains is the latency between the two
 // halves of a row (warps wait for loads 5 of 14 cycles). The row held in shared memory behind bulk copies, its clusters of
 // 8 exchanging sums, took 1,016 us: an exchange costs 2 us a row.
@@ -958,7 +961,7 @@ __device__ __forceinline__ float softplus_neg(float x) { return log1pf(expf(-fab
 constexpr int kPairThreads = 1024;
 // One block, split into teams of threads: a team sums the log-probabilities of a pair's two sequences (in 64 bits, in a
 // fixed order), its first thread works out the pair's loss, and the team writes the rows' coefficients. Tens of thousands
-// of rows are a few hundred kilobytes, so one block's time stays far below the logits' (8,000 rows: 12 us beside 430).
+// of rows are a few hundred kilobytes, so one block's time stays far below the logits' (8,000 rows: 15 us beside 430).
 __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const PreferenceArgs a) {
   griddep_wait();  // launched with programmatic stream serialization (launch_pdl)
   griddep_launch_dependents();
