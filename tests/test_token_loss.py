@@ -277,3 +277,16 @@ def test_large_logits_over_temperature(dtype, temperature, top):
     _, want, want_h = oracle.rows(x, tokens, torch.ones(8, dtype=torch.bool), temperature)
     assert ((logp.double() - want).abs() <= oracle.logp_bound(want)).all()
     assert ((entropy.double() - want_h).abs() <= 2 * oracle.logp_bound(want_h) + 2e-5).all()
+
+
+def test_rows_outside_the_sequences_hold_anything():
+    logits, tokens, *_ = _case((12,), seed=6)
+    spoiled = logits.clone()
+    spoiled[:2], spoiled[10], spoiled[11, 3] = float("nan"), float("inf"), float("-inf")
+    offsets = torch.tensor([2, 5, 5, 7, 10])
+    clean, want = preference_loss_grad(logits, tokens, offsets=offsets)
+    out, grad = preference_loss_grad(spoiled, tokens, offsets=offsets)
+    assert torch.equal(out.loss, clean.loss) and torch.equal(grad, want)
+    assert (grad[:2] == 0).all() and (grad[10:] == 0).all()
+    none, grad = preference_loss_grad(spoiled, tokens, offsets=torch.tensor([3]))
+    assert none.loss == 0 and (grad == 0).all()

@@ -256,6 +256,10 @@ def _preference_settings(beta, label_smoothing, loss_type, average):
 def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind, average, temperature):
     ref, mask = _constant(ref), _constant(mask)
     w = _row_weights(logits, tokens, mask)
+    if logits.dim() == 2 and offsets is not None and offsets.dim() == 1 and offsets.numel():
+        # rows before the first and behind the last sequence get no gradient, whatever they hold
+        row, ends = torch.arange(len(w)), offsets.long()
+        logits = torch.where(((row >= ends[0]) & (row < ends[-1]))[:, None], logits, logits.detach())
     logp, _ = _logprobs_torch(logits, tokens, w, temperature)
     weighted = (w * logp).double()
     if logits.dim() == 3:
