@@ -290,3 +290,26 @@ def test_rows_outside_the_sequences_hold_anything():
     assert (grad[:2] == 0).all() and (grad[10:] == 0).all()
     none, grad = preference_loss_grad(spoiled, tokens, offsets=torch.tensor([3]))
     assert none.loss == 0 and (grad == 0).all()
+
+
+def clipped_ratios(device):
+    """A ratio beyond fp32's range (the old policy all but excluded the token) is clipped like any other: no gradient where
+    the advantage is positive, an infinite loss where it is not."""
+    logits, tokens, old, adv, *_ = (x.to(device) for x in _case((6,), seed=7))
+    for far in (-100.0, float("-inf")):
+        old[2] = far
+        adv[2] = 1.5
+        out, grad = token_policy_loss_grad(logits, tokens, old, adv)
+        rest = torch.arange(6, device=device) != 2
+        other, want = token_policy_loss_grad(logits, tokens, old, adv, mask=rest, reduction="sum")
+        assert out.loss.item() == pytest.approx((other.loss.item() - 1.5 * 1.2) / 6, rel=1e-5, abs=1e-6)
+        assert torch.allclose(grad, want / 6, rtol=1e-5, atol=1e-7) and (grad[2] == 0).all()
+        z = logits.clone().requires_grad_()
+        token_policy_loss(z, tokens, old, adv).loss.backward()
+        assert torch.allclose(z.grad, grad, rtol=1e-4, atol=1e-6)
+        adv[2] = -1.5
+        assert token_policy_loss_grad(logits, tokens, old, adv)[0].loss == float("inf")
+
+
+def test_clipped_ratios():
+    clipped_ratios("cpu")

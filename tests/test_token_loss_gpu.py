@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import token_oracle as oracle
-from test_token_loss import (RANGES, REFUSALS, decided_pairs, extreme_rows, only_logits_get_gradients, refuse,
-                             refuse_preference)
+from test_token_loss import (RANGES, REFUSALS, clipped_ratios, decided_pairs, extreme_rows, only_logits_get_gradients,
+                             refuse, refuse_preference)
 from tt_rsl_rl_b200.ops.token_loss import (preference_loss, preference_loss_grad, token_logprobs, token_policy_loss,
                                            token_policy_loss_grad)
 
@@ -564,3 +564,7 @@ def test_preference_losses(dtype, kind, smoothing, average):
                              offsets=torch.arange(0, 73, 9).cuda(), **(kwargs | {"mask": mask.cuda().flatten()})).loss]
     for got in forms:
         assert abs(got.item() - loss) <= tol
+
+
+def test_clipped_ratios():
+    clipped_ratios("cuda")

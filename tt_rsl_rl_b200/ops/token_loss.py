@@ -156,10 +156,14 @@ def _policy_torch(logits, tokens, old, adv, ref, mask, lo, hi, kl_coef, kl_kind,
     w = _row_weights(logits, tokens, mask)
     counted = w != 0
     logp, entropy = _logprobs_torch(logits, tokens, w, temperature)
-    ratio = torch.exp(torch.where(counted, logp - old, 0.0))
     neg_adv = torch.where(counted, -adv, 0.0)
-    free, cut = neg_adv * ratio, neg_adv * ratio.clamp(lo, hi)
-    surrogate = torch.max(free, cut)
+    with torch.no_grad():
+        ratio = torch.exp(torch.where(counted, logp - old, 0.0))
+        free, cut = neg_adv * ratio, neg_adv * ratio.clamp(lo, hi)
+        open_ = (free > cut) | free.isnan() | ((ratio >= lo) & (ratio <= hi))
+    # a clipped ratio passes no gradient, an infinite one neither
+    moving = torch.where(open_, logp, logp.detach())
+    surrogate = torch.where(open_, neg_adv * torch.exp(torch.where(counted, moving - old, 0.0)), cut)
     kl = torch.zeros_like(logp)
     if ref is not None:
         d = torch.where(counted, ref - logp, 0.0)
