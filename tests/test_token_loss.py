@@ -313,3 +313,10 @@ def clipped_ratios(device):
 
 def test_clipped_ratios():
     clipped_ratios("cpu")
+
+
+def test_decreasing_offsets_are_refused():
+    logits, tokens, *_ = _case((20,), seed=8)
+    for offsets in ([0, 10, 5, 20, 20], [5, 3, 20], [0, 10, 30, 15, 20]):
+        with pytest.raises(ValueError, match="decrease"):
+            preference_loss_grad(logits, tokens, offsets=torch.tensor(offsets))

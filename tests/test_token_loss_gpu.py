@@ -568,3 +568,18 @@ def test_preference_losses(dtype, kind, smoothing, average):
 
 def test_clipped_ratios():
     clipped_ratios("cuda")
+
+
+def test_decreasing_offsets_give_nan():
+    """Two sequences may not share a row: the kernel says so, since the host does not wait for the offsets."""
+    x, tokens, mask, _ = _make((4000,), 40, torch.float32, seed=16)
+    mask = mask.cuda()
+    many = torch.arange(0, 4001, 2)
+    many[1990] = many[1988] - 1
+    for offsets in ([0, 10, 5, 20, 20], [5, 3, 20], many.tolist(), [0, 10, 5000, 3999, 4000]):
+        out, grad = preference_loss_grad(x.cuda(), tokens.cuda(), offsets=torch.tensor(offsets).cuda(), mask=mask)
+        assert out.loss.isnan() and all(t.isnan().all() for t in out[1:4])
+        assert grad[mask].isnan().all() and (grad[~mask] == 0).all()
+        z = x.cuda().requires_grad_()
+        preference_loss(z, tokens.cuda(), offsets=torch.tensor(offsets).cuda().int(), mask=mask).loss.backward()
+        assert z.grad[mask].isnan().all()

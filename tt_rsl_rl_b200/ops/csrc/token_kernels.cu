@@ -968,6 +968,11 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
   __shared__ double s_part[kPairThreads / 32][4];
   __shared__ float s_coef[kPairThreads / 32][2];
   __shared__ double s_loss[kPairThreads / 32];
+  // Offsets that decrease would give a row to two teams. They are not known to the host, so what they lead to is a NaN.
+  int bad = 0;  // looked at where the first pair's sums meet, so that these loads hide behind the rows'
+  if (a.offsets != nullptr) {
+    for (int64_t s = threadIdx.x; s < a.seqs; s += kPairThreads) bad |= seq_start(a, s + 1) < seq_start(a, s);
+  }
   for (int64_t r = threadIdx.x; r < a.rows; r += kPairThreads) a.coef[r] = 0.f;
   const int64_t pairs = a.seqs / 2;
   int teams = 1;
@@ -1007,7 +1012,14 @@ __global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pr
     for (int n = 0; n < 4; ++n) {
       for (int o = 16; o >= 1; o >>= 1) x[n] += __shfl_xor_sync(0xffffffffu, x[n], o);
     }
-    __syncthreads();  // the rows are cleared, the last pairs' partial sums and coefficients have been read
+    // the rows are cleared, the last pairs' partial sums and coefficients have been read
+    if (__syncthreads_or(bad)) {
+      const float none = nanf("");
+      for (int64_t r = threadIdx.x; r < a.rows; r += kPairThreads) a.coef[r] = none;
+      for (int64_t s = threadIdx.x; s < a.seqs; s += kPairThreads) a.seq_logp[s] = a.rewards[s] = none;
+      if (threadIdx.x == 0) a.loss[0] = none;
+      return;
+    }
     if (lane == 0) {
       for (int n = 0; n < 4; ++n) s_part[warp][n] = x[n];
     }

@@ -278,6 +278,8 @@ def _preference_torch(logits, tokens, ref, offsets, mask, beta, smoothing, kind,
         if offsets.dim() != 1 or offsets.numel() < 1:
             raise ValueError("offsets must be [sequences + 1]")
         at = offsets.long().clamp(0, len(w)).tolist()
+        if any(a > b for a, b in zip(at[:-1], at[1:])):
+            raise ValueError("offsets must not decrease")
         parts = [(weighted[a:b].sum(), w[a:b].double().sum()) for a, b in zip(at[:-1], at[1:])]
         sums, counts = (torch.stack(x) for x in zip(*parts)) if parts else (weighted[:0], weighted[:0])
     if len(sums) % 2:
@@ -314,7 +316,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logps: torch
     A sequence's log-probability is the weighted sum (``average=True``: mean) of its rows' ``logp``, summed in 64 bits.
     ``[sequences, rows, V]`` logits hold one sequence per batch entry; packed ``[rows, V]`` logits come with ``offsets``
     ``[sequences + 1]``, non-decreasing row numbers on the same device (values outside ``[0, rows]`` are clamped; rows
-    before the first and behind the last sequence get a zero gradient). ``ref_logps`` are the sequences'
+    before the first and behind the last sequence get a zero gradient; where they decrease, CPU tensors raise an error, and
+    on CUDA, where the host does not wait for them, loss, rewards and gradients are NaN). ``ref_logps`` are the sequences'
     log-probabilities under the reference (None: zero). With ``h`` the difference of ``beta (logp - ref)``, a pair's loss
     is ``-(1 - s) log sigmoid(h) - s log sigmoid(-h)`` (``"sigmoid"``, ``s`` the label smoothing), ``max(0, 1 - h)``
     (``"hinge"``) or ``(h / beta - 1 / (2 beta))^2`` (``"ipo"``)."""
